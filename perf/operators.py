@@ -242,9 +242,10 @@ def _inputs(case, seed, cache=None, prefix=None):
 
 
 class _DeviceArray:
-    """An executor's device buffer as torch sees it."""
+    """An executor's device buffer as torch sees it; a tensor made of it keeps the executor, whose memory it is."""
 
     def __init__(self, executor, is_output, index):
+        self.executor = executor
         array = (executor.host_outputs if is_output else executor.host_inputs)[index]
         pointer, _ = executor.device_buffer(is_output, index)
         self.__cuda_array_interface__ = {"shape": array.shape, "typestr": array.dtype.str, "data": (pointer, False), "version": 3}
