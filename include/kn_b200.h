@@ -223,6 +223,27 @@ KN_API void kn_comm_destroy(kn_comm* comm);
 /* Attaches `comm` (may be NULL: back to a world of one) to the executor.  Not while an evaluation is in flight. */
 KN_API int kn_executor_set_comm(kn_executor* exec, kn_comm* comm);
 
+/* Decoders that answer token by token.  No counterpart in the reference, whose executor keeps nothing between evaluations.
+ *
+ * A graph may contain caches (operation tag 17 of the blob): keys and values of the positions of several sequences, which
+ * its cache writes (18) add to and its cache reads (19) and attention (20) use.  Their storage is made by the host, outlives
+ * every evaluation, and is attached to each executor that works on it: the one that takes in a prompt and the one that
+ * answers, say.  `sequences`, `heads`, `capacity`, `dim` and `dtype` (the tag of i8 or f16) are those of the graph's cache at
+ * the executor's batch size; positions never written are 0.  An evaluation with a cache that is not attached is an error.
+ *
+ * Executors of one device may share a cache; what one has enqueued comes before what another enqueues later, whatever their
+ * streams.  They are used by one thread at a time then.  kn_cache_destroy gives up the handle; the memory lives as
+ * long as an executor has it attached. */
+typedef struct kn_cache kn_cache;
+KN_API int kn_cache_create(int device, size_t sequences, size_t heads, size_t capacity, size_t dim, int dtype, kn_cache** out);
+KN_API void kn_cache_destroy(kn_cache* cache);
+/* Device memory that it takes. */
+KN_API int kn_cache_bytes(const kn_cache* cache, uint64_t* bytes);
+KN_API int kn_executor_cache_count(const kn_executor* exec, int* n_caches);
+/* Attaches `cache` (NULL: none) as the graph's cache number `index`.  Waits for the executor's stream; not while an evaluation is in
+ * flight.  One cache cannot stand for two of a graph's. */
+KN_API int kn_executor_set_cache(kn_executor* exec, int index, kn_cache* cache);
+
 /* Self-test of the bounded waits, with no counterpart in the reference.  Every barrier wait inside the
  * tensor-core kernels gives up after a cycle limit, raises the executor's status word and lets the
  * kernel return, and the next synchronising call reports KN_ERR_INTERNAL.  In normal operation no wait

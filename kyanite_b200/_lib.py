@@ -71,6 +71,11 @@ SIGNATURES = {
     "kn_comm_create": (c_int, [c_int, c_int, c_int, c_void_p, c_size_t, POINTER(c_void_p)]),
     "kn_comm_destroy": (None, [c_void_p]),
     "kn_executor_set_comm": (c_int, [c_void_p, c_void_p]),
+    "kn_cache_create": (c_int, [c_int, c_size_t, c_size_t, c_size_t, c_size_t, c_int, POINTER(c_void_p)]),
+    "kn_cache_destroy": (None, [c_void_p]),
+    "kn_cache_bytes": (c_int, [c_void_p, POINTER(c_uint64)]),
+    "kn_executor_cache_count": (c_int, [c_void_p, POINTER(c_int)]),
+    "kn_executor_set_cache": (c_int, [c_void_p, c_int, c_void_p]),
     "kn_executor_selftest_wait_expiry": (c_int, [c_void_p, c_uint32]),
     "kn_matmul_tf32_static": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p]),
     "kn_matmul_tf32_static_status": (c_int, [POINTER(c_int)]),

@@ -44,6 +44,9 @@ SOURCES = [
     "kernels/attn_softmax.cu",
     "kernels/attention.cu",
     "kernels/flash.cu",
+    "kernels/cache.cu",
+    "kernels/cache_attention.cu",
+    "kernels/sample.cu",
 ]
 
 NVCC_FLAGS = [

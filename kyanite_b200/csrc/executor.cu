@@ -9,6 +9,7 @@
 #include <cstring>
 #include <functional>
 #include <memory>
+#include <mutex>
 #include <sstream>
 #include <string>
 #include <vector>
@@ -86,6 +87,25 @@ constexpr size_t kMinOutputSetBytes = 64 << 10;
 // Inputs of up to this many bytes in all go up, and outputs of up to as many come down, by a kernel (host_copy.cu).
 constexpr size_t kKernelTransferBytes = 64 << 10;
 
+struct Executor;
+
+// Storage of a decoder's cache: attached to the executors that write and read it, which keep it alive
+struct CacheStorage {
+    int device = 0;
+    DType dtype = DType::I8;
+    CacheParams params{};
+    size_t bytes = 0;
+    std::mutex mu;
+    Executor* last = nullptr;          // whose stream has its latest work, if that executor lives
+    ~CacheStorage() {
+        int prev = -1;
+        cudaGetDevice(&prev);
+        cudaSetDevice(device);
+        if (params.base) cudaFree(params.base);
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
 struct Executor {
     int device = 0;
     std::unique_ptr<Plan> plan;
@@ -109,6 +129,7 @@ struct Executor {
     std::vector<float> step_us;
     int launches = 0;                            // of one run of all steps
     std::vector<DenseChainParams> dense_runs;    // of plan->dense_runs
+    std::vector<std::shared_ptr<CacheStorage>> caches;   // of plan->caches; null until attached
     Comm* comm = nullptr;              // not owned; AllReduce steps sum over its ranks (null: a world of one)
 
     ~Executor() {
@@ -117,6 +138,7 @@ struct Executor {
         cudaGetDevice(&prev);
         cudaSetDevice(device);
         if (stream) cudaStreamSynchronize(stream);
+        for (auto& c : caches) leave(c);
         if (graph_exec) cudaGraphExecDestroy(graph_exec);
         drop_eval_graphs();
         if (side_stream) cudaStreamDestroy(side_stream);
@@ -135,15 +157,64 @@ struct Executor {
         eval_graphs.clear();
     }
 
+    // Whoever uses the cache next need not wait for this executor's stream, which is done
+    void leave(const std::shared_ptr<CacheStorage>& c) {
+        if (!c) return;
+        std::lock_guard<std::mutex> lock(c->mu);
+        if (c->last == this) c->last = nullptr;
+    }
+
+    // Before work that uses the caches goes to the stream: all are attached, and what another executor has enqueued on one
+    // of them comes first.  (Nothing to do while one executor uses them.)
+    void enter_caches() {
+        for (size_t i = 0; i < caches.size(); i++) {
+            KN_CHECK(caches[i] != nullptr, KN_ERR_INVALID_ARG, "no cache is attached as cache " + std::to_string(i) + " (kn_executor_set_cache)");
+            CacheStorage& c = *caches[i];
+            std::lock_guard<std::mutex> lock(c.mu);
+            if (c.last == this) continue;
+            if (c.last != nullptr) {
+                cudaEvent_t e;
+                KN_CUDA(cudaEventCreateWithFlags(&e, cudaEventDisableTiming));
+                cudaError_t err = cudaEventRecord(e, c.last->stream);
+                if (err == cudaSuccess) err = cudaStreamWaitEvent(stream, e, 0);
+                cudaEventDestroy(e);
+                KN_CUDA(err);
+            }
+            c.last = this;
+        }
+    }
+
+    void set_cache(size_t index, std::shared_ptr<CacheStorage> c) {
+        KN_CUDA(cudaStreamSynchronize(stream));
+        // graphs captured with the previous storage would go on using it
+        if (graph_exec) { cudaGraphExecDestroy(graph_exec); graph_exec = nullptr; }
+        drop_eval_graphs();
+        leave(caches[index]);
+        caches[index] = std::move(c);
+        patch_pointers(true);
+    }
+
     uint8_t* device_ptr(const PlanTensor& t) const {
         const BufferInfo& b = plan->buffers[t.buf];
+        if (b.kind == BufKind::Cache) return caches[b.cache] ? caches[b.cache]->params.base : nullptr;
         uint8_t* base = b.kind == BufKind::Const ? consts : arena;
         return base + b.arena_offset + t.offset * dtype_size(t.dtype);
     }
 
-    void patch_pointers() {
-        launches = 0;
+    // The cache behind an operand, with its pointers (null until it is attached)
+    CacheParams cache_at(const CacheParams& planned, const PlanTensor& t) const {
+        CacheParams c = planned;
+        const auto& storage = caches[plan->buffers[t.buf].cache];
+        c.base = storage ? storage->params.base : nullptr;
+        c.scales = storage ? storage->params.scales : nullptr;
+        return c;
+    }
+
+    // `of_caches`: only the steps that use caches, which have been attached meanwhile
+    void patch_pointers(bool of_caches = false) {
+        if (!of_caches) launches = 0;
         for (Step& s : plan->steps) {
+            if (of_caches && s.kind != StepKind::CacheWrite && s.kind != StepKind::CacheRead && s.kind != StepKind::CacheAttention) continue;
             std::vector<void*> ptr;
             for (auto& t : s.operands) ptr.push_back(device_ptr(t));
             switch (s.kind) {
@@ -220,6 +291,52 @@ struct Executor {
                     s.all_reduce.in = ptr[0];
                     s.all_reduce.out = ptr[1];
                     break;
+                case StepKind::CacheWrite: {
+                    CacheWriteParams& p = s.cache_write;
+                    p.cache = cache_at(p.cache, s.operands[0]);
+                    p.in[0] = ptr[1], p.in[1] = ptr[2];
+                    p.start = (const int32_t*)ptr[3];
+                    p.count = ptr.size() > 4 ? (const int32_t*)ptr[4] : nullptr;
+                    break;
+                }
+                case StepKind::CacheRead:
+                    s.cache_read.cache = cache_at(s.cache_read.cache, s.operands[0]);
+                    s.cache_read.out = ptr[1];
+                    break;
+                case StepKind::CacheAttention: {   // query, cache, out, start, then those that are there
+                    CacheAttentionParams& p = s.cache_attention;
+                    const OptionalOperands& has = s.optional;
+                    p.cache = cache_at(p.cache, s.operands[1]);
+                    p.query = ptr[0];
+                    p.out = ptr[2];
+                    p.start = (const int32_t*)ptr[3];
+                    size_t at = 4;
+                    if (has.count) p.count = (const int32_t*)ptr[at++];
+                    if (has.slopes) p.slopes = (const float*)ptr[at++];
+                    if (has.prefix) {
+                        p.prefix = cache_at(p.prefix, s.operands[at++]);
+                        p.prefix_length = (const int32_t*)ptr[at++];
+                    }
+                    if (at < ptr.size()) {
+                        p.partial = (float*)ptr[at++];
+                        p.arrived = (uint32_t*)ptr[at++];
+                    }
+                    p.status = status_dev;
+                    break;
+                }
+                case StepKind::Sample: {
+                    SampleParams& p = s.sample;
+                    const OptionalOperands& has = s.optional;
+                    p.logits = ptr[0];
+                    p.out = (int32_t*)ptr[1];
+                    p.uniform = (const float*)ptr[2];
+                    size_t at = 3;
+                    if (has.temperature) p.temperature = (const float*)ptr[at++];
+                    if (has.top_k) p.top_k = (const int32_t*)ptr[at++];
+                    if (has.top_p) p.top_p = (const float*)ptr[at++];
+                    if (has.min_p) p.min_p = (const float*)ptr[at++];
+                    break;
+                }
                 case StepKind::ConvChain:
                     s.chain.in = (const float*)ptr[0];
                     s.chain.out = (float*)ptr[1];
@@ -231,9 +348,9 @@ struct Executor {
             }
             if (s.tensor_core || s.kind == StepKind::ConvChain)
                 tc_prepare_step(s, status_dev, plan->opts.flags, (plan->opts.flags & KN_FLAG_TRACE_GEMM) ? status_host + 4 : nullptr);
-            launches += s.launches;
+            if (!of_caches) launches += s.launches;
         }
-        prepare_dense_runs();
+        if (!of_caches) prepare_dense_runs();
     }
 
     // What the runs of dense layers are launched with (Plan::dense_runs).  The steps stay what they are for whoever times them one by one.
@@ -297,6 +414,10 @@ struct Executor {
             case StepKind::Im2col: err = launch_im2col(s.im2col, stream); break;
             case StepKind::RmsNorm: err = launch_rmsnorm(s.rms, stream); break;
             case StepKind::GroupNorm: err = launch_group_norm(s.group_norm, stream); break;
+            case StepKind::CacheWrite: err = launch_cache_write(s.cache_write, stream); break;
+            case StepKind::CacheRead: err = launch_cache_read(s.cache_read, stream); break;
+            case StepKind::CacheAttention: err = launch_cache_attention(s.cache_attention, stream); break;
+            case StepKind::Sample: err = launch_sample(s.sample, stream); break;
             case StepKind::AllReduce: {
                 const AllReduceParams& a = s.all_reduce;
                 if (comm != nullptr && comm->world > 1)
@@ -314,6 +435,7 @@ struct Executor {
 
     void run_async() {
         if (plan->steps.empty()) return;
+        enter_caches();
         if (profile) {
             std::vector<cudaEvent_t> ev(plan->steps.size() + 1, nullptr);
             try {
@@ -541,6 +663,7 @@ struct Executor {
         KN_CHECK(!in_flight, KN_ERR_INVALID_ARG, "evaluate_begin while an evaluation is in flight");
         for (size_t i = 0; i < pinned_in.size(); i++)
             KN_CHECK(inputs != nullptr && (inputs[i] != nullptr || bytes_in[i] == 0), KN_ERR_INVALID_ARG, "null input buffer");
+        enter_caches();
         settle();
         staging_busy = true;
         const bool graph = use_graph() && !profile;
@@ -648,6 +771,7 @@ static std::unique_ptr<Executor> create_executor(int device, const Graph& graph,
         ex->bytes_out.push_back(bytes);
         ex->dtype_out.push_back(plan.outputs[i].dtype);
     }
+    ex->caches.resize(plan.caches.size());
     KN_CUDA(cudaMemsetAsync(ex->arena, 0, std::max<size_t>(plan.arena_bytes, 256), ex->stream));
     ex->patch_pointers();
     KN_CUDA(cudaStreamSynchronize(ex->stream));
@@ -670,6 +794,9 @@ struct kn_outputs {
 };
 struct kn_comm {
     kn::Comm* c = nullptr;
+};
+struct kn_cache {
+    std::shared_ptr<kn::CacheStorage> c;
 };
 
 namespace {
@@ -963,6 +1090,7 @@ int kn_executor_time_step(kn_executor* exec, int step, int launches, float* micr
         KN_CHECK(step >= 0 && (size_t)step < e.plan->steps.size(), KN_ERR_INVALID_ARG, "step index out of range");
         KN_CHECK(launches >= 1 && launches <= 100000, KN_ERR_INVALID_ARG, "launch count out of range");
         kn::DeviceGuard guard(e.device);
+        e.enter_caches();
         cudaEvent_t a, b;
         KN_CUDA(cudaEventCreate(&a));
         KN_CUDA(cudaEventCreate(&b));
@@ -1024,6 +1152,72 @@ int kn_executor_set_comm(kn_executor* exec, kn_comm* comm) {
         if (e.graph_exec) { cudaGraphExecDestroy(e.graph_exec); e.graph_exec = nullptr; }
         e.drop_eval_graphs();
         e.comm = comm ? comm->c : nullptr;
+    });
+}
+
+int kn_cache_create(int device, size_t sequences, size_t heads, size_t capacity, size_t dim, int dtype, kn_cache** out) {
+    return guarded([&] {
+        KN_CHECK(out != nullptr, KN_ERR_INVALID_ARG, "null out pointer");
+        *out = nullptr;
+        KN_CHECK(sequences >= 1 && heads >= 1 && capacity >= 1 && dim >= 1 && dim <= (size_t)kn::kCacheMaxDim, KN_ERR_INVALID_ARG,
+                 "a cache has at least one sequence, head and position and 1 to 256 channels");
+        KN_CHECK(sequences < (1u << 30) && heads < (1u << 30) && capacity < (1u << 30) && (double)sequences * heads * capacity * 2048 < 9e18, KN_ERR_INVALID_ARG, "a cache that large");
+        KN_CHECK(dtype == (int)kn::DType::I8 || dtype == (int)kn::DType::F16, KN_ERR_INVALID_ARG, "a cache holds i8 or f16");
+        int count = 0;
+        if (cudaGetDeviceCount(&count) != cudaSuccess) cudaGetLastError(), count = 0;
+        KN_CHECK(device >= 0 && device < count, KN_ERR_NO_DEVICE, "CUDA device " + std::to_string(device) + " not available");
+        kn::DeviceGuard guard(device);
+        auto c = std::make_shared<kn::CacheStorage>();
+        c->device = device;
+        c->dtype = (kn::DType)dtype;
+        c->params = kn::cache_params((int64_t)sequences, (int64_t)heads, (int64_t)capacity, (int64_t)dim, c->dtype);
+        c->bytes = (size_t)kn::cache_bytes(c->params);
+        cudaError_t err = cudaMalloc((void**)&c->params.base, c->bytes);
+        if (err != cudaSuccess) {
+            c->params.base = nullptr;
+            cudaGetLastError();
+            kn::fail(KN_ERR_CUDA, "no device memory for a cache of " + std::to_string(c->bytes) + " bytes: " + cudaGetErrorString(err));
+        }
+        if (!c->params.half) c->params.scales = (float*)(c->params.base + kn::cache_rows(c->params) * c->params.row_bytes);
+        KN_CUDA((cudaError_t)kn::cache_clear_async(c->params, nullptr));
+        KN_CUDA(cudaStreamSynchronize(nullptr));
+        *out = new kn_cache{std::move(c)};
+    });
+}
+
+void kn_cache_destroy(kn_cache* cache) { delete cache; }
+
+int kn_cache_bytes(const kn_cache* cache, uint64_t* bytes) {
+    return guarded([&] {
+        KN_CHECK(cache != nullptr && bytes != nullptr, KN_ERR_INVALID_ARG, "null argument");
+        *bytes = cache->c->bytes;
+    });
+}
+
+int kn_executor_cache_count(const kn_executor* exec, int* n_caches) {
+    return guarded([&] {
+        KN_CHECK(exec != nullptr && n_caches != nullptr, KN_ERR_INVALID_ARG, "null argument");
+        *n_caches = (int)exec->e->caches.size();
+    });
+}
+
+int kn_executor_set_cache(kn_executor* exec, int index, kn_cache* cache) {
+    return guarded([&] {
+        KN_CHECK(exec != nullptr, KN_ERR_INVALID_ARG, "null executor");
+        kn::Executor& e = *exec->e;
+        KN_CHECK(index >= 0 && (size_t)index < e.caches.size(), KN_ERR_INVALID_ARG, "cache index out of range");
+        KN_CHECK(!e.in_flight, KN_ERR_INVALID_ARG, "an evaluation is in flight");
+        kn::DeviceGuard guard(e.device);
+        if (cache != nullptr) {
+            KN_CHECK(cache->c->device == e.device, KN_ERR_INVALID_ARG, "cache and executor are on different devices");
+            const kn::PlanTensor& t = e.plan->caches[index];
+            const kn::CacheParams& c = cache->c->params;
+            const std::vector<int64_t> has{2, c.seqs, c.heads, c.capacity, c.dim};
+            KN_CHECK(t.ss.shape == has && t.dtype == cache->c->dtype, KN_ERR_SHAPE, "the graph's cache has another shape or dtype: " + t.str());
+            for (size_t i = 0; i < e.caches.size(); i++)
+                KN_CHECK((int)i == index || e.caches[i] != cache->c, KN_ERR_INVALID_ARG, "the same cache is attached as cache " + std::to_string(i));
+        }
+        e.set_cache((size_t)index, cache != nullptr ? cache->c : nullptr);
     });
 }
 

@@ -16,7 +16,8 @@ const char* dtype_name(DType d) {
 
 const char* op_name(OpKind k) {
     static const char* names[] = {"Input", "Constant", "View", "Broadcast", "Permute", "Slice", "Flip", "Gather",
-                                  "Concat", "Conv", "MatMul", "Unary", "Binary", "Softmax", "Layernorm", "Reduce", "AllReduce"};
+                                  "Concat", "Conv", "MatMul", "Unary", "Binary", "Softmax", "Layernorm", "Reduce", "AllReduce",
+                                  "Cache", "CacheWrite", "CacheRead", "CacheAttention", "Sample"};
     return (int)k < (int)OpKind::COUNT ? names[(int)k] : "?";
 }
 
@@ -68,6 +69,15 @@ int checked_operand(Reader& r, size_t current) {
     uint32_t v = r.u32();
     KN_CHECK(v < current, KN_ERR_BAD_GRAPH, "graph blob: operand does not precede its user");
     return (int)v;
+}
+
+// 0xffffffff: none; else appended to `inputs`.  Returns its position there, or -1
+int optional_operand(Reader& r, size_t current, std::vector<int>& inputs) {
+    uint32_t v = r.u32();
+    if (v == 0xffffffffu) return -1;
+    KN_CHECK(v < current, KN_ERR_BAD_GRAPH, "graph blob: operand does not precede its user");
+    inputs.push_back((int)v);
+    return (int)inputs.size() - 1;
 }
 
 }  // namespace
@@ -215,8 +225,55 @@ std::unique_ptr<Graph> Graph::parse(const void* bytes, size_t len) {
                 for (uint32_t k = 0; k < n; k++) info.axes.push_back((int)r.u32());
                 break;
             }
+            case OpKind::Cache:
+                info.input_index = (int)r.u32();
+                KN_CHECK(info.input_index == (int)g->caches.size(), KN_ERR_BAD_GRAPH, "graph blob: caches are not numbered in order");
+                KN_CHECK(rank == 5 && (info.dtype == DType::I8 || info.dtype == DType::F16), KN_ERR_BAD_GRAPH, "graph blob: a cache has five axes of i8 or f16");
+                g->caches.push_back((int)i);
+                break;
+            case OpKind::CacheWrite:
+                for (int k = 0; k < 4; k++) info.inputs.push_back(checked_operand(r, i));
+                info.count_at = optional_operand(r, i, info.inputs);
+                KN_CHECK(info.dtype == g->values[info.inputs[0]].dtype, KN_ERR_BAD_GRAPH, "graph blob: a written cache keeps its dtype");
+                break;
+            case OpKind::CacheRead:
+                info.inputs = {checked_operand(r, i)};
+                KN_CHECK(info.dtype == DType::F32 || info.dtype == DType::F16, KN_ERR_BAD_GRAPH, "graph blob: a cache is read as f32 or f16");
+                break;
+            case OpKind::CacheAttention: {
+                for (int k = 0; k < 3; k++) info.inputs.push_back(checked_operand(r, i));
+                info.count_at = optional_operand(r, i, info.inputs);
+                info.slopes_at = optional_operand(r, i, info.inputs);
+                info.prefix_at = optional_operand(r, i, info.inputs);
+                info.prefix_length_at = optional_operand(r, i, info.inputs);
+                info.scale = r.take<float>();
+                info.softcap = r.take<float>();
+                info.window = r.u32();
+                const DType d = g->values[info.inputs[0]].dtype;
+                KN_CHECK(d == info.dtype && (d == DType::F32 || d == DType::F16), KN_ERR_BAD_GRAPH, "graph blob: attention takes f32 or f16 and keeps the dtype");
+                KN_CHECK((info.prefix_at < 0) == (info.prefix_length_at < 0), KN_ERR_BAD_GRAPH, "graph blob: a prefix and its length come together");
+                KN_CHECK(std::isfinite(info.scale) && std::isfinite(info.softcap) && info.softcap >= 0.f && info.window < (1u << 31), KN_ERR_BAD_GRAPH,
+                         "graph blob: attention scale, softcap or window");
+                break;
+            }
+            case OpKind::Sample: {
+                for (int k = 0; k < 2; k++) info.inputs.push_back(checked_operand(r, i));
+                info.temperature_at = optional_operand(r, i, info.inputs);
+                info.top_k_at = optional_operand(r, i, info.inputs);
+                info.top_p_at = optional_operand(r, i, info.inputs);
+                info.min_p_at = optional_operand(r, i, info.inputs);
+                const DType d = g->values[info.inputs[0]].dtype;
+                KN_CHECK(info.dtype == DType::I32 && (d == DType::F32 || d == DType::F16), KN_ERR_BAD_GRAPH, "graph blob: sampling takes f32 or f16 and gives i32");
+                break;
+            }
             default:
                 fail(KN_ERR_BAD_GRAPH, "graph blob: unknown operation");
+        }
+        // caches: taken only where they belong, and where they belong nothing else
+        for (size_t k = 0; k < info.inputs.size(); k++) {
+            const bool wanted = ((info.op == OpKind::CacheWrite || info.op == OpKind::CacheRead) && k == 0) ||
+                                (info.op == OpKind::CacheAttention && (k == 1 || (int)k == info.prefix_at));
+            KN_CHECK(is_cache(g->values[info.inputs[k]].op) == wanted, KN_ERR_BAD_GRAPH, std::string("graph blob: operand of ") + op_name(info.op) + (wanted ? " is no cache" : " is a cache"));
         }
         // axis sanity against the operand rank
         if (!info.inputs.empty()) {
@@ -242,6 +299,10 @@ std::unique_ptr<Graph> Graph::parse(const void* bytes, size_t len) {
         g->values.push_back(std::move(info));
     }
     KN_CHECK(r.pos == len, KN_ERR_BAD_GRAPH, "graph blob: trailing bytes");
+    for (const ValueInfo& info : g->values)
+        KN_CHECK(info.op != OpKind::CacheWrite || g->values[info.inputs[0]].non_output_uses == 1, KN_ERR_BAD_GRAPH,
+                 "graph blob: a cache that is written has another user");
+    for (int v : g->outputs) KN_CHECK(!is_cache(g->values[v].op), KN_ERR_BAD_GRAPH, "graph blob: a cache is an output");
     for (size_t k = 0; k < g->inputs.size(); k++) {
         const ValueInfo& info = g->values[g->inputs[k]];
         KN_CHECK(info.op == OpKind::Input && info.input_index == (int)k, KN_ERR_BAD_GRAPH,

@@ -10,11 +10,14 @@ namespace kn {
 
 // 0..15 are the reference's `Operation` variants (kn-graph/src/graph.rs:106-162); AllReduce is an extension
 // for tensor-parallel graphs (the reference runs one graph on one device): the element-wise sum of the value
-// over the ranks of the communicator attached to the executor, the value itself when there is none.
+// over the ranks of the communicator attached to the executor, the value itself when there is none.  The last five are
+// extensions for decoders that answer token by token: Cache is storage that is attached to the executor and outlives an
+// evaluation, CacheWrite the same storage once something is written into it.
 enum class OpKind : uint8_t {
     Input = 0, Constant, View, Broadcast, Permute, Slice, Flip, Gather, Concat, Conv, MatMul, Unary, Binary,
-    Softmax, Layernorm, Reduce, AllReduce, COUNT
+    Softmax, Layernorm, Reduce, AllReduce, Cache, CacheWrite, CacheRead, CacheAttention, Sample, COUNT
 };
+inline bool is_cache(OpKind k) { return k == OpKind::Cache || k == OpKind::CacheWrite; }
 const char* op_name(OpKind k);
 
 // `factor * batch^exp` (kn-graph/src/shape.rs:37-44)
@@ -40,7 +43,7 @@ struct ValueInfo {
     std::vector<Size> shape;
     std::vector<int> inputs;
 
-    int input_index = 0;                       // Input
+    int input_index = 0;                       // Input Cache
     const uint8_t* const_data = nullptr;       // Constant: points into Graph::blob
     size_t const_bytes = 0;
     std::vector<int> permutation;              // Permute
@@ -53,6 +56,11 @@ struct ValueInfo {
     ReduceOp reduce_op = ReduceOp::Sum;
     std::vector<int> axes;                     // Reduce
     float eps = 0.f;                           // Layernorm
+    // CacheWrite, CacheAttention, Sample: positions in `inputs` of the operands that may be left out, or -1
+    int count_at = -1, slopes_at = -1, prefix_at = -1, prefix_length_at = -1;   // CacheWrite (count) CacheAttention
+    int temperature_at = -1, top_k_at = -1, top_p_at = -1, min_p_at = -1;       // Sample
+    float scale = 0.f, softcap = 0.f;          // CacheAttention
+    uint32_t window = 0;                       // CacheAttention: 0 none
 
     int non_output_uses = 0;                   // recomputed on load (graph.rs:549-552)
 };
@@ -60,7 +68,7 @@ struct ValueInfo {
 struct Graph {
     std::vector<uint8_t> blob;                 // owns constant payloads
     std::vector<ValueInfo> values;
-    std::vector<int> inputs, outputs;
+    std::vector<int> inputs, outputs, caches;
 
     static std::unique_ptr<Graph> parse(const void* bytes, size_t len);
 

@@ -287,6 +287,68 @@ struct AllReduceParams {
     uint8_t dtype;     // DType: F32 or F16
 };
 
+// ---- the cache of a decoder: keys and values of every position of every sequence.  Storage (kn_cache_create): rows of `row_bytes`,
+// one per part (0 keys, 1 values), sequence, head and position, in that order, `padded` positions to a head; behind them, of an
+// i8 cache, their scales in the same order.  A row holds the channels, padded to a multiple of 64 with zeros, as f16 or as whole
+// numbers + 128, in 16-byte chunks whose order depends on the position (kernels/cache.cuh).
+constexpr int kCacheMaxDim = 256, kCachePositions = 64;   // capacities are padded to a multiple of these
+struct CacheParams {
+    uint8_t* base;
+    float* scales;           // null: f16
+    int64_t part_rows;       // rows between keys and values
+    int32_t seqs, heads, capacity, padded, dim, row_bytes, half;
+};
+int64_t cache_rows(const CacheParams& c);      // rows in all
+int64_t cache_bytes(const CacheParams& c);     // of all of it
+CacheParams cache_params(int64_t seqs, int64_t heads, int64_t capacity, int64_t dim, DType dtype);   // without pointers
+int cache_clear_async(const CacheParams& c, cudaStream_t stream);   // all zeros
+
+// New tokens into the cache: token t of sequence s at position start[s] + t, the first count[s] of them
+struct CacheWriteParams {
+    CacheParams cache;
+    const void* in[2];             // keys, values: [seqs][tokens][heads][dim]
+    int64_t strides[2][4];         // in elements
+    const int32_t *start, *count;  // count may be null
+    int32_t tokens, half;          // half: `in` holds f16
+};
+// All of the cache as numbers: [2][seqs][heads][capacity][dim], dense
+struct CacheReadParams {
+    CacheParams cache;
+    void* out;
+    int32_t half;
+};
+// softmax(scores) . values of new tokens against the cache (kernels/cache_attention.cu)
+struct CacheAttentionParams {
+    CacheParams cache, prefix;     // prefix.base null: none
+    const void* query;             // [seqs][tokens][heads][dim]
+    void* out;                     // the same, dense
+    int64_t q_strides[4];          // in elements
+    const int32_t *start, *count, *prefix_length;
+    const float* slopes;           // per query head, or null
+    float* partial;                // results of parts of a row's keys, for the CTA that joins them
+    uint32_t* arrived;             // per item: parts that are done; all 0 between launches
+    uint32_t* status;              // word that the kernel raises when a bounded wait expires
+    float scale, softcap;
+    int32_t window, tokens, heads, half;
+    int32_t grid;                  // CTAs (cache_attention_plan)
+};
+struct CacheAttentionPlan {
+    int32_t grid;
+    int64_t items, partial_floats;
+};
+CacheAttentionPlan cache_attention_plan(const CacheAttentionParams& p);
+
+// ---- one token for every row of logits (kernels/sample.cu)
+constexpr int64_t kSampleMaxVocab = 1 << 19;
+struct SampleParams {
+    const void* logits;            // [rows][vocab], f32 or f16
+    const float *uniform, *temperature, *top_p, *min_p;   // per row; all but the first may be null
+    const int32_t* top_k;          // may be null
+    int32_t* out;
+    int64_t rows, row_stride, col_stride;
+    int32_t vocab, half;
+};
+
 // ---- small transfers between device memory and pinned host memory (kernels/host_copy.cu)
 constexpr int kMaxHostCopies = 8;
 struct HostCopyParams {
@@ -316,5 +378,9 @@ constexpr int64_t kSoftmaxMatmulMaxKeys = 128, kSoftmaxMatmulMaxCols = 128;
 int launch_softmax_matmul(const GemmParams& p, cudaStream_t stream);   // p.row_softmax == 4
 int launch_conv_simt(const ConvParams& p, cudaStream_t stream);
 int launch_host_copy(const HostCopyParams& p, cudaStream_t stream);
+int launch_cache_write(const CacheWriteParams& p, cudaStream_t stream);   // kernels/cache.cu
+int launch_cache_read(const CacheReadParams& p, cudaStream_t stream);
+int launch_cache_attention(const CacheAttentionParams& p, cudaStream_t stream);
+int launch_sample(const SampleParams& p, cudaStream_t stream);
 
 }  // namespace kn

@@ -16,7 +16,8 @@
 namespace kn {
 
 const char* step_kind_name(StepKind k) {
-    static const char* names[] = {"Scalar", "Reduce", "Softmax", "Layernorm", "Gather", "Gemm", "Conv", "ConvChain", "Im2col", "AllReduce", "RmsNorm", "GroupNorm"};
+    static const char* names[] = {"Scalar", "Reduce", "Softmax", "Layernorm", "Gather", "Gemm", "Conv", "ConvChain", "Im2col", "AllReduce", "RmsNorm", "GroupNorm",
+                                  "CacheWrite", "CacheRead", "CacheAttention", "Sample"};
     return (int)k < (int)StepKind::COUNT ? names[(int)k] : "?";
 }
 
@@ -178,12 +179,15 @@ class Planner {
         plan_.inputs.resize(g_.inputs.size());
         // every graph input gets a buffer, used or not (planner.rs:117-121)
         for (int v : g_.inputs) visit(v);
+        for (int v : g_.caches) plan_.caches.push_back(visit(v));
         for (int v : g_.outputs) {
             PlanTensor t = ensure_simple(visit(v), v);
             buffer(t.buf).always_live = true;
             plan_.outputs.push_back(t);
             plan_.output_shapes.push_back(t.ss.shape);
         }
+        for (size_t v = 0; v < g_.values.size(); v++)   // (caches are written whether or not an output depends on it)
+            if (g_.values[v].op == OpKind::CacheWrite) visit((int)v);
         for (auto& t : plan_.inputs) plan_.input_shapes.push_back(t.ss.shape);
         fuse_conv_chains();
         drop_unused_constants();
@@ -658,8 +662,179 @@ class Planner {
                 }
                 return out;
             }
+            case OpKind::Cache: {
+                const CacheParams c = cache_of(v);
+                BufferInfo b;
+                b.kind = BufKind::Cache;
+                b.bytes = (size_t)cache_bytes(c);
+                b.value = v;
+                b.cache = info.input_index;
+                plan_.buffers.push_back(b);
+                PlanTensor t;
+                t.buf = (int)plan_.buffers.size() - 1;
+                t.dtype = info.dtype;
+                t.ss = StridedShape::simple(shape);
+                return t;
+            }
+            case OpKind::CacheWrite: return visit_cache_write(v);
+            case OpKind::CacheRead: return visit_cache_read(v);
+            case OpKind::CacheAttention: return visit_cache_attention(v);
+            case OpKind::Sample: return visit_sample(v);
             default: fail(KN_ERR_INTERNAL, "unknown operation");
         }
+    }
+
+    // ---------------------------------------------------------------- a decoder's cache, attention to it, sampling
+    CacheParams cache_of(int v) const {
+        const std::vector<int64_t> d = shape_of(v);
+        KN_CHECK(d.size() == 5 && d[0] == 2 && d[2] >= 1 && d[3] >= 1 && d[4] >= 1 && d[4] <= kCacheMaxDim, KN_ERR_SHAPE, "a cache is [2][sequences][heads][capacity][1 to 256 channels]");
+        for (int64_t n : d) KN_CHECK(n < (1 << 30), KN_ERR_SHAPE, "a cache's axis is too long");
+        KN_CHECK((double)d[1] * d[2] * d[3] * 2048 < 9e18, KN_ERR_SHAPE, "a cache is too large");
+        return cache_params(d[1], d[2], d[3], d[4], g_.values[v].dtype);
+    }
+
+    // One number per entry, in memory one behind the other
+    PlanTensor vector_operand(int v, int64_t n, DType dtype, const char* what) {
+        KN_CHECK(shape_of(v) == std::vector<int64_t>{n} && g_.values[v].dtype == dtype, KN_ERR_SHAPE, std::string(what) + ": wrong shape or dtype");
+        return ensure_simple(visit(v), v);
+    }
+
+    PlanTensor visit_cache_write(int v) {
+        const ValueInfo& info = g_.values[v];
+        PlanTensor cache = visit(info.inputs[0]);
+        Step s;
+        s.kind = StepKind::CacheWrite;
+        s.value = v;
+        CacheWriteParams& p = s.cache_write;
+        p.cache = cache_of(info.inputs[0]);
+        KN_CHECK(shape_of(v) == shape_of(info.inputs[0]), KN_ERR_SHAPE, "a written cache keeps its shape");
+        s.operands = {cache};
+        s.writes = {1};
+        for (int k = 0; k < 2; k++) {
+            const PlanTensor in = visit(info.inputs[1 + k]);
+            const std::vector<int64_t>& d = in.ss.shape;
+            KN_CHECK(d.size() == 4 && d[0] == p.cache.seqs && d[2] == p.cache.heads && d[3] == p.cache.dim && d[1] < (1 << 30) &&
+                         (in.dtype == DType::F32 || in.dtype == DType::F16) && (k == 0 || (d == s.operands[1].ss.shape && in.dtype == s.operands[1].dtype)),
+                     KN_ERR_SHAPE, "cache write: keys and values are f32 or f16, [sequences][tokens][heads][channels]");
+            p.tokens = (int)d[1];
+            p.half = in.dtype == DType::F16;
+            for (int i = 0; i < 4; i++) p.strides[k][i] = in.ss.strides[i];
+            s.operands.push_back(in);
+            s.writes.push_back(0);
+        }
+        s.operands.push_back(vector_operand(info.inputs[3], p.cache.seqs, DType::I32, "cache write: start"));
+        s.writes.push_back(0);
+        if (info.count_at >= 0) {
+            s.operands.push_back(vector_operand(info.inputs[info.count_at], p.cache.seqs, DType::I32, "cache write: count"));
+            s.writes.push_back(0);
+        }
+        s.desc = "cachewrite seqs=" + std::to_string(p.cache.seqs) + " tokens=" + std::to_string(p.tokens) + " heads=" + std::to_string(p.cache.heads) + " dim=" +
+                 std::to_string(p.cache.dim) + (p.half ? " f16" : " f32") + " into " + dtype_name(info.dtype);
+        if ((int64_t)p.tokens * p.cache.seqs == 0) return cache;
+        const double row = p.cache.dim * (p.cache.half ? 2.0 : 1.0) + (p.cache.half ? 0 : 4);
+        push_step(std::move(s));
+        Step& pushed = plan_.steps.back();
+        pushed.alg_bytes = 2.0 * pushed.cache_write.tokens * pushed.cache_write.cache.seqs * pushed.cache_write.cache.heads *
+                           (row + pushed.cache_write.cache.dim * (pushed.cache_write.half ? 2.0 : 4.0));
+        return cache;
+    }
+
+    PlanTensor visit_cache_read(int v) {
+        const ValueInfo& info = g_.values[v];
+        PlanTensor cache = visit(info.inputs[0]);
+        PlanTensor out = alloc_shared(shape_of(v), info.dtype, v);
+        Step s;
+        s.kind = StepKind::CacheRead;
+        s.value = v;
+        s.operands = {cache, out};
+        s.writes = {0, 1};
+        s.cache_read.cache = cache_of(info.inputs[0]);
+        s.cache_read.half = info.dtype == DType::F16;
+        s.desc = std::string("cacheread ") + dtype_name(cache.dtype) + " as " + dtype_name(info.dtype) + " count=" + std::to_string(out.ss.size());
+        if (out.ss.size() != 0) push_step(std::move(s));
+        return out;
+    }
+
+    PlanTensor visit_cache_attention(int v) {
+        const ValueInfo& info = g_.values[v];
+        const PlanTensor q = visit(info.inputs[0]);
+        const PlanTensor cache = visit(info.inputs[1]);
+        PlanTensor out = alloc_shared(shape_of(v), info.dtype, v);
+        Step s;
+        s.kind = StepKind::CacheAttention;
+        s.value = v;
+        CacheAttentionParams& p = s.cache_attention;
+        p.cache = cache_of(info.inputs[1]);
+        const std::vector<int64_t>& d = q.ss.shape;
+        KN_CHECK(d.size() == 4 && d == out.ss.shape && d[0] == p.cache.seqs && d[3] == p.cache.dim && d[1] < (1 << 30) && d[2] >= 1 && d[2] < (1 << 30) && d[2] % p.cache.heads == 0,
+                 KN_ERR_SHAPE, "cache attention: the query is [sequences][tokens][a multiple of the cache's heads][channels]");
+        p.tokens = (int)d[1], p.heads = (int)d[2];
+        p.half = q.dtype == DType::F16;
+        for (int i = 0; i < 4; i++) p.q_strides[i] = q.ss.strides[i];
+        p.scale = info.scale, p.softcap = info.softcap, p.window = (int)info.window;
+        s.operands = {q, cache, out};
+        auto add = [&](const PlanTensor& t, int writes) {
+            s.operands.push_back(t);
+            s.writes.push_back((uint8_t)writes);
+        };
+        s.writes = {0, 0, 1};
+        add(vector_operand(info.inputs[2], p.cache.seqs, DType::I32, "cache attention: start"), 0);
+        if (info.count_at >= 0) add(vector_operand(info.inputs[info.count_at], p.cache.seqs, DType::I32, "cache attention: count"), 0);
+        if (info.slopes_at >= 0) add(vector_operand(info.inputs[info.slopes_at], p.heads, DType::F32, "cache attention: slopes"), 0);
+        if (info.prefix_at >= 0) {
+            const int pv = info.inputs[info.prefix_at];
+            p.prefix = cache_of(pv);
+            KN_CHECK(p.prefix.seqs == 1 && p.prefix.heads == p.cache.heads && p.prefix.dim == p.cache.dim && p.prefix.half == p.cache.half, KN_ERR_SHAPE,
+                     "cache attention: the prefix is a cache of one sequence with the other's heads, channels and dtype");
+            add(visit(pv), 0);
+            add(vector_operand(info.inputs[info.prefix_length_at], 1, DType::I32, "cache attention: prefix length"), 0);
+        }
+        if (out.ss.size() == 0) return out;
+        KN_CHECK((int64_t)p.tokens * p.heads * p.cache.seqs < (1ll << 31), KN_ERR_UNSUPPORTED, "cache attention: too many rows");
+        const CacheAttentionPlan plan = cache_attention_plan(p);
+        p.grid = plan.grid;
+        if (plan.partial_floats) {
+            add(alloc_shared({plan.partial_floats}, DType::F32, v), 1);
+            PlanTensor arrived = alloc_shared({plan.items}, DType::U32, v);
+            buffer(arrived.buf).always_live = true;   // (zero between launches)
+            add(arrived, 1);
+        }
+        s.optional.count = info.count_at >= 0, s.optional.slopes = info.slopes_at >= 0, s.optional.prefix = info.prefix_at >= 0;
+        // what it needs where every sequence is as long as the cache
+        const double keys = (double)p.cache.capacity + (p.prefix.dim ? p.prefix.capacity : 0);
+        s.flops = 4.0 * p.cache.seqs * p.tokens * p.heads * p.cache.dim * keys;
+        s.desc = "cacheattention seqs=" + std::to_string(p.cache.seqs) + " tokens=" + std::to_string(p.tokens) + " heads=" + std::to_string(p.heads) + "/" +
+                 std::to_string(p.cache.heads) + " dim=" + std::to_string(p.cache.dim) + " capacity=" + std::to_string(p.cache.capacity) +
+                 (info.prefix_at >= 0 ? " prefix=" + std::to_string(p.prefix.capacity) : "") + (p.half ? " f16" : " f32") + " cache " + dtype_name(cache.dtype);
+        push_step(std::move(s));
+        return out;
+    }
+
+    PlanTensor visit_sample(int v) {
+        const ValueInfo& info = g_.values[v];
+        const PlanTensor logits = visit(info.inputs[0]);
+        PlanTensor out = alloc_shared(shape_of(v), DType::I32, v);
+        const std::vector<int64_t>& d = logits.ss.shape;
+        KN_CHECK(d.size() == 2 && out.ss.shape == std::vector<int64_t>{d[0]} && d[1] >= 1 && d[1] <= kSampleMaxVocab, KN_ERR_SHAPE, "sampling takes [rows][1 to 2^19 tokens] and gives [rows]");
+        KN_CHECK(d[0] < (1ll << 31), KN_ERR_UNSUPPORTED, "sampling: too many rows");
+        Step s;
+        s.kind = StepKind::Sample;
+        s.value = v;
+        SampleParams& p = s.sample;
+        p.rows = d[0], p.vocab = (int)d[1], p.half = logits.dtype == DType::F16;
+        p.row_stride = logits.ss.strides[0], p.col_stride = logits.ss.strides[1];
+        s.operands = {logits, out, vector_operand(info.inputs[1], d[0], DType::F32, "sampling: uniform")};
+        s.writes = {0, 1, 0};
+        for (int at : {info.temperature_at, info.top_k_at, info.top_p_at, info.min_p_at})
+            if (at >= 0) {
+                s.operands.push_back(vector_operand(info.inputs[at], d[0], at == info.top_k_at ? DType::I32 : DType::F32, "sampling: a parameter"));
+                s.writes.push_back(0);
+            }
+        s.optional.temperature = info.temperature_at >= 0, s.optional.top_k = info.top_k_at >= 0, s.optional.top_p = info.top_p_at >= 0;
+        s.optional.min_p = info.min_p_at >= 0;
+        s.desc = "sample rows=" + std::to_string(d[0]) + " vocab=" + std::to_string(d[1]) + (p.half ? " f16" : " f32");
+        if (d[0] != 0) push_step(std::move(s));
+        return out;
     }
 
     // Where a concatenation goes: channels-last if it joins the channels of images that all are (each part is a copy of whole

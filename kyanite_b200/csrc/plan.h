@@ -14,7 +14,7 @@
 
 namespace kn {
 
-enum class BufKind : uint8_t { Const, Shared, Zero };
+enum class BufKind : uint8_t { Const, Shared, Zero, Cache };   // Cache: attached to the executor
 
 struct BufferInfo {
     BufKind kind = BufKind::Shared;
@@ -23,7 +23,8 @@ struct BufferInfo {
     const uint8_t* host_data = nullptr;   // Const: bytes to upload (points into the graph blob or `owned`)
     std::shared_ptr<std::vector<uint8_t>> owned;   // Const data produced by the planner itself
     int first_step = 1 << 30, last_step = -1;
-    bool always_live = false;          // graph inputs and outputs
+    bool always_live = false;          // graph inputs and outputs, what a kernel leaves for its next launch
+    int cache = -1;                    // Cache: its number
     int64_t arena_offset = -1;         // Shared: byte offset inside the arena; Const: inside the constant block
 };
 
@@ -49,8 +50,15 @@ struct PlanTensor {
 
 struct TcLaunch;   // tensor maps and launch geometry of a tensor-core step (kernels/contract_tc.cu)
 
-enum class StepKind : uint8_t { Scalar = 0, Reduce, Softmax, Layernorm, Gather, Gemm, Conv, ConvChain, Im2col, AllReduce, RmsNorm, GroupNorm, COUNT };
+enum class StepKind : uint8_t { Scalar = 0, Reduce, Softmax, Layernorm, Gather, Gemm, Conv, ConvChain, Im2col, AllReduce, RmsNorm, GroupNorm,
+                                CacheWrite, CacheRead, CacheAttention, Sample, COUNT };
 const char* step_kind_name(StepKind k);
+
+// Which of the operands that may be left out a step has
+struct OptionalOperands {
+    bool count = false, slopes = false, prefix = false;                       // CacheAttention
+    bool temperature = false, top_k = false, top_p = false, min_p = false;   // Sample
+};
 
 struct Step {
     StepKind kind = StepKind::Scalar;
@@ -75,6 +83,11 @@ struct Step {
     AllReduceParams all_reduce{};
     RmsNormParams rms{};
     GroupNormParams group_norm{};
+    CacheWriteParams cache_write{};
+    CacheReadParams cache_read{};
+    CacheAttentionParams cache_attention{};
+    SampleParams sample{};
+    OptionalOperands optional{};
 };
 
 // Steps that are launched together: a run of small dense layers and the softmax behind them, if there is one (kernels/dense_chain.cu)
@@ -92,6 +105,7 @@ struct Plan {
     std::vector<PlanTensor> inputs;    // dense, one per graph input
     std::vector<PlanTensor> outputs;   // dense, one per graph output
     std::vector<std::vector<int64_t>> input_shapes, output_shapes;
+    std::vector<PlanTensor> caches;    // by number
     size_t arena_bytes = 0, const_bytes = 0, zero_bytes = 0;
     int collectives = 0;               // AllReduce steps
     kn_mem_usage mem{};

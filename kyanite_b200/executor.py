@@ -23,7 +23,7 @@ from . import _lib
 from ._lib import KnError, KnMemUsage, KnOptions, KnTensorInfo, check
 from .graph import DType, Graph
 
-__all__ = ["Communicator", "CudaDevice", "CudaDeviceNotAvailable", "CudaExecutor", "Device", "PreparedGraph", "MemoryUsage",
+__all__ = ["Communicator", "CudaDevice", "CudaDeviceNotAvailable", "CudaExecutor", "Device", "KvCache", "PreparedGraph", "MemoryUsage",
            "plan_describe", "KnError", "MATH_TF32", "MATH_F32", "FLAG_NO_CONV_CHAIN", "FLAG_NO_PERSISTENT_GEMM"]
 
 MATH_TF32 = _lib.KN_MATH_TF32
@@ -160,6 +160,42 @@ class Communicator:
     def close(self):
         if getattr(self, "_ptr", None):
             self._lib.kn_comm_destroy(self._ptr)
+            self._ptr = c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KvCache:
+    """Keys and values of a decoder's sequences, in device memory that outlives evaluations (kn_cache_create): the storage behind
+    a `Graph.cache` of the same sizes, attached with `CudaExecutor.set_cache` to every executor that writes or reads it.
+    `dtype`: I8 (a scale per position and head) or F16.  Positions never written are 0."""
+
+    def __init__(self, device, sequences: int, heads: int, capacity: int, dim: int, dtype: DType = DType.I8):
+        self._lib = _lib.load()
+        self._ptr = c_void_p()
+        self.device = device.index if isinstance(device, CudaDevice) else int(device)
+        self.shape, self.dtype = (2, int(sequences), int(heads), int(capacity), int(dim)), DType(dtype)
+        if min(self.shape) < 1:
+            raise ValueError(f"a cache has at least one of everything, got {self.shape[1:]}")
+        status = self._lib.kn_cache_create(self.device, *self.shape[1:], int(self.dtype), byref(self._ptr))
+        if status == 6:
+            raise CudaDeviceNotAvailable(self._lib.kn_last_error().decode())
+        check(status)
+
+    @property
+    def nbytes(self) -> int:
+        """Device memory that it takes."""
+        n = c_uint64()
+        check(self._lib.kn_cache_bytes(self._ptr, byref(n)))
+        return n.value
+
+    def close(self):
+        if getattr(self, "_ptr", None):
+            self._lib.kn_cache_destroy(self._ptr)
             self._ptr = c_void_p()
 
     def __del__(self):
@@ -349,6 +385,19 @@ class CudaExecutor:
         """Attaches the communicator the graph's all-reduce values sum over (None: a world of one rank)."""
         check(self._lib.kn_executor_set_comm(self._ptr, comm._ptr if comm is not None else None))
         self._comm = comm   # keep it alive as long as the executor uses it
+
+    def set_cache(self, index: int, cache: Optional["KvCache"]):
+        """Attaches the storage of the graph's cache number `index` (None: none).  An evaluation needs all of them; executors that
+        share one work on it in the order of their calls."""
+        if cache is not None and not cache._ptr:
+            raise ValueError("the cache has been closed")
+        check(self._lib.kn_executor_set_cache(self._ptr, int(index), cache._ptr if cache is not None else None))
+
+    @property
+    def cache_count(self) -> int:
+        n = c_int()
+        check(self._lib.kn_executor_cache_count(self._ptr, byref(n)))
+        return n.value
 
     def upload_inputs(self):
         check(self._lib.kn_executor_upload_inputs(self._ptr))

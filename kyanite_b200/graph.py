@@ -292,6 +292,12 @@ class OpKind(enum.IntEnum):
     LAYERNORM = 14
     REDUCE = 15
     ALL_REDUCE = 16    # extension (no counterpart in the reference): sum over the ranks of a communicator
+    # extensions for decoders that answer token by token (no counterpart in the reference)
+    CACHE = 17              # keys and values that outlive an evaluation: storage attached to the executor
+    CACHE_WRITE = 18
+    CACHE_READ = 19
+    CACHE_ATTENTION = 20
+    SAMPLE = 21
 
 
 @dataclass(frozen=True)
@@ -322,6 +328,8 @@ class ValueInfo:
     reduce_op: Optional[ReduceOp] = None
     axes: Tuple[int, ...] = ()                 # REDUCE
     eps: float = 0.0                           # LAYERNORM
+    present: Tuple[bool, ...] = ()             # CACHE_WRITE CACHE_ATTENTION SAMPLE: which of the optional operands `inputs` has
+    attention: Tuple[float, float, int] = (0.0, 0.0, 0)   # CACHE_ATTENTION: scale, softcap, window
     debug_id: str = ""
     non_output_uses: int = 0
 
@@ -332,7 +340,7 @@ class ValueInfo:
         eps_bits = struct.pack("<f", self.eps)
         return (self.shape, self.dtype, self.kind, self.inputs, self.input_index, t, self.permutation,
                 self.axis, self.range, self.conv, self.unary_op, self.cast_to, self.binary_op,
-                self.reduce_op, self.axes, eps_bits)
+                self.reduce_op, self.axes, eps_bits, self.present, self.attention)
 
 
 _next_check = [1]
@@ -349,6 +357,7 @@ class Graph:
         self._back_map = {}
         self.inputs: List[Value] = []
         self.outputs: List[Value] = []
+        self.caches: List[Value] = []
 
     # ---------------------------------------------------------------- basic access
     def __getitem__(self, v: Value) -> ValueInfo:
@@ -510,6 +519,8 @@ class Graph:
         for i in info.inputs:
             if i >= len(self.values):
                 raise ValueError("operand does not belong to this graph")
+        self._check_caches(info)
+        for i in info.inputs:
             self.values[i].non_output_uses += 1
         index = len(self.values)
         self.values.append(info)
@@ -823,6 +834,145 @@ class Graph:
             raise ValueError(f"all_reduce takes f32 or f16, got {d}")
         return self._push(ValueInfo(s, d, OpKind.ALL_REDUCE, inputs=(input.index,)))
 
+    # ---------------------------------------------------------------- decoders: cache, attention to it, sampling
+    def cache(self, sequences, heads: int, capacity: int, dim: int, dtype: DType = DType.I8) -> Value:
+        """Extension: keys and values of up to `capacity` positions of each of `sequences` sequences, `heads` heads of `dim`
+        channels, that outlive an evaluation.  Their storage is a `KvCache` of the same sizes that the program attaches to the
+        executor (`CudaExecutor.set_cache`, by the order in which a graph's caches are made).  `dtype`: I8, whole numbers with
+        one f32 scale per position and head (scale = max|x| / 127, x read back as round(x / scale) * scale, rounding half
+        to even), or F16.  Only cache_write, cache_read and cache_attention take the value, of shape
+        [2 (keys, values), sequences, heads, capacity, dim]."""
+        if dtype not in (DType.I8, DType.F16):
+            raise ValueError(f"a cache holds I8 or F16, got {dtype!r}")
+        heads, capacity, dim = int(heads), int(capacity), int(dim)
+        if not (1 <= dim <= 256 and heads >= 1 and 1 <= capacity < 1 << 30):
+            raise ValueError(f"a cache has at least one head, 1 to 256 channels and 1 to 2^30 - 1 positions, got {heads}, {dim}, {capacity}")
+        return self._push_cache(ValueInfo(shape((2, sequences, heads, capacity, dim)), dtype, OpKind.CACHE))
+
+    def _push_cache(self, info: ValueInfo) -> Value:
+        v = self._push(ValueInfo(info.shape, info.dtype, OpKind.CACHE, input_index=len(self.caches)))
+        self.caches.append(v)
+        return v
+
+    def _check_caches(self, info: ValueInfo):
+        """Caches are only taken by the operations that know them, and one that is written has no other user: every reader takes
+        what the write returns, so that the order of reading and writing is the graph's."""
+        takes = {OpKind.CACHE_WRITE: (0,), OpKind.CACHE_READ: (0,), OpKind.CACHE_ATTENTION: (1, self._prefix_operand(info))}
+        for position, i in enumerate(info.inputs):
+            if self.values[i].kind not in (OpKind.CACHE, OpKind.CACHE_WRITE):
+                continue
+            if position not in takes.get(info.kind, ()):
+                raise ValueError(f"{info.kind.name} does not take a cache")
+            writes = info.kind == OpKind.CACHE_WRITE
+            if (writes and self.values[i].non_output_uses) or any(x.kind == OpKind.CACHE_WRITE and x.inputs[0] == i for x in self.values):
+                raise ValueError("a cache that is written has no other user: read what cache_write returns")
+
+    @staticmethod
+    def _prefix_operand(info: ValueInfo) -> int:
+        count, slopes, prefix = (tuple(info.present) + (False,) * 3)[:3]
+        return 3 + count + slopes if prefix else -1
+
+    def _cache_shape(self, cache: Value):
+        info = self[cache]
+        if info.kind not in (OpKind.CACHE, OpKind.CACHE_WRITE):
+            raise ValueError("Expected a cache, or what cache_write returns")
+        return info.shape
+
+    def _check_vector(self, v: Optional[Value], size: Size, dtype: DType, what: str):
+        if v is None:
+            return
+        if tuple(self[v].shape) != (size,) or self[v].dtype != dtype:
+            raise ValueError(f"{what} must be {dtype.name} of shape ({size},), got {self[v].dtype.name} {self[v].shape}")
+
+    def cache_write(self, cache: Value, keys: Value, values: Value, start: Value, count: Optional[Value] = None) -> Value:
+        """Extension: writes `keys` and `values` [sequences, tokens, heads, dim], f32 or f16, into the cache: token t of
+        sequence s at position start[s] + t (I32).  Of a padded batch only the first count[s] tokens are written.  Positions
+        outside the cache are dropped; everything else stays as it is.  Returns the written cache.  A graph writes its
+        caches whether or not an output depends on them."""
+        _, sequences, heads, _, dim = self._cache_shape(cache)
+        for x in (keys, values):
+            s, d = self.shape_dtype(x)
+            if len(s) != 4 or (s[0], s[2], s[3]) != (sequences, heads, dim) or d not in (DType.F32, DType.F16) or self[x].kind in (OpKind.CACHE, OpKind.CACHE_WRITE):
+                raise ValueError(f"keys and values must be f32 or f16 of shape ({sequences}, tokens, {heads}, {dim}), got {d.name} {s}")
+        if self.shape_dtype(keys) != self.shape_dtype(values):
+            raise ValueError("keys and values must have the same shape and dtype")
+        self._check_vector(start, sequences, DType.I32, "start")
+        self._check_vector(count, sequences, DType.I32, "count")
+        inputs = (cache, keys, values, start) + ((count,) if count is not None else ())
+        return self._push(ValueInfo(self[cache].shape, self[cache].dtype, OpKind.CACHE_WRITE, inputs=tuple(v.index for v in inputs),
+                                    present=(count is not None,)))
+
+    def cache_read(self, cache: Value, dtype: DType = DType.F16) -> Value:
+        """Extension: what the cache holds, as numbers: [2, sequences, heads, capacity, dim] in f16 or f32.  Positions
+        never written are 0."""
+        s = self._cache_shape(cache)
+        if dtype not in (DType.F32, DType.F16):
+            raise ValueError(f"a cache is read as F32 or F16, got {dtype!r}")
+        return self._push(ValueInfo(s, dtype, OpKind.CACHE_READ, inputs=(cache.index,)))
+
+    def cache_attention(self, query: Value, cache: Value, start: Value, count: Optional[Value] = None, scale: Optional[float] = None,
+                        softcap: float = 0.0, window: int = 0, slopes: Optional[Value] = None, prefix: Optional[Value] = None,
+                        prefix_length: Optional[Value] = None) -> Value:
+        """Extension: softmax(scores) . values for `query` [sequences, tokens, heads, dim], f32 or f16; the result has its
+        shape and dtype.  `heads` is a multiple of the cache's, of which each serves as many neighbouring query heads.
+
+        Token t of sequence s is at position start[s] + t (I32) and sees the positions up to its own, its own among them.  With
+        `prefix`, a cache of one sequence, the first prefix_length[0] (I32) positions of it are in front of every
+        sequence.  score = scale * q . k (default 1 / sqrt(dim)); then softcap * tanh(score / softcap) if `softcap` is not 0;
+        then, with `slopes` (f32, one per query head), minus slope * distance.  With `window`, only positions less
+        than that far away are seen.  Of a padded batch the first count[s] tokens count; the others, and tokens that see no
+        position (before 0, behind the capacity), get zeros."""
+        qs, qd = self.shape_dtype(query)
+        _, sequences, kv_heads, _, dim = self._cache_shape(cache)
+        if len(qs) != 4 or qd not in (DType.F32, DType.F16) or (qs[0], qs[3]) != (sequences, dim) or self[query].kind in (OpKind.CACHE, OpKind.CACHE_WRITE):
+            raise ValueError(f"query must be f32 or f16 of shape ({sequences}, tokens, heads, {dim}), got {qd.name} {qs}")
+        heads = qs[2].unwrap_fixed("heads")
+        if heads < 1 or heads % kv_heads.unwrap_fixed("heads"):
+            raise ValueError(f"{heads} query heads are not a multiple of the cache's {kv_heads}")
+        self._check_vector(start, sequences, DType.I32, "start")
+        self._check_vector(count, sequences, DType.I32, "count")
+        self._check_vector(slopes, qs[2], DType.F32, "slopes")
+        if (prefix is None) != (prefix_length is None):
+            raise ValueError("prefix and prefix_length come together")
+        if prefix is not None:
+            ps = self._cache_shape(prefix)
+            if (ps[1], ps[2], ps[4]) != (ONE, kv_heads, dim) or self[prefix].dtype != self[cache].dtype:
+                raise ValueError("prefix must be a cache of one sequence with the other's heads, dim and dtype")
+            self._check_vector(prefix_length, ONE, DType.I32, "prefix_length")
+        scale = float(np.float32(1.0 / math.sqrt(dim.unwrap_fixed("dim")) if scale is None else scale))
+        softcap, window = float(np.float32(softcap)), int(window)
+        if not (math.isfinite(scale) and math.isfinite(softcap) and softcap >= 0 and 0 <= window < 1 << 31):
+            raise ValueError("scale must be finite, softcap finite and not negative, window from 0 to 2^31 - 1")
+        optional = (count, slopes, prefix)
+        inputs = [query, cache, start] + [v for v in optional + (prefix_length,) if v is not None]
+        return self._push(ValueInfo(qs, qd, OpKind.CACHE_ATTENTION, inputs=tuple(v.index for v in inputs),
+                                    present=tuple(v is not None for v in optional), attention=(scale, softcap, window)))
+
+    def sample(self, logits: Value, uniform: Value, temperature: Optional[Value] = None, top_k: Optional[Value] = None,
+               top_p: Optional[Value] = None, min_p: Optional[Value] = None) -> Value:
+        """Extension: one token (I32) for every row of `logits` [rows, vocabulary], f32 or f16, by random numbers that the
+        caller gives: `uniform` (f32, from 0 up to but not 1), one per row.  The others are per row too, each may be left out.
+
+        A token weighs exp((logit - highest logit) / temperature).  In falling order of the logits, the lowest index first among
+        equals: the first top_k (I32; 0 or less: all) stay; of these the fewest that have top_p of their weight (1 or more: all);
+        of these the ones that weigh at least min_p.  The first always stays.  Then, in the order of the index, the first token behind
+        which more than uniform of the remaining weight lies.  Weights count in steps of 2^-44 of the highest.  Temperature 0
+        (or less): the highest logit, the lowest index among equals.  NaN counts as -infinity; a row with nothing else
+        gives -1.  Of logits of +infinity each weighs 1 and all others 0."""
+        s, d = self.shape_dtype(logits)
+        if len(s) != 2 or d not in (DType.F32, DType.F16) or self[logits].kind in (OpKind.CACHE, OpKind.CACHE_WRITE):
+            raise ValueError(f"logits must be f32 or f16 of rank 2, got {d.name} {s}")
+        vocab = s[1].unwrap_fixed("vocabulary")
+        if not 1 <= vocab <= 1 << 19:
+            raise ValueError(f"vocabularies have 1 to 2^19 tokens, got {vocab}")
+        for v, dtype, what in ((uniform, DType.F32, "uniform"), (temperature, DType.F32, "temperature"), (top_k, DType.I32, "top_k"),
+                               (top_p, DType.F32, "top_p"), (min_p, DType.F32, "min_p")):
+            self._check_vector(v, s[0], dtype, what)
+        optional = (temperature, top_k, top_p, min_p)
+        inputs = [logits, uniform] + [v for v in optional if v is not None]
+        return self._push(ValueInfo((s[0],), DType.I32, OpKind.SAMPLE, inputs=tuple(v.index for v in inputs),
+                                    present=tuple(v is not None for v in optional)))
+
     # ---------------------------------------------------------------- elementwise
     def sigmoid(self, input: Value) -> Value:
         return self.unary(UnaryOp.SIGMOID, input)
@@ -909,6 +1059,8 @@ class Graph:
         for i, info in enumerate(graph.values):
             if info.kind == OpKind.INPUT:
                 mapping[i] = inputs[info.input_index]
+            elif info.kind == OpKind.CACHE:      # a cache of this graph's own
+                mapping[i] = self._push_cache(info)
             else:
                 copy = ValueInfo(**{**info.__dict__, "inputs": tuple(mapping[j].index for j in info.inputs),
                                     "non_output_uses": 0, "debug_id": ""})
@@ -917,6 +1069,8 @@ class Graph:
 
     def output(self, v: Value):
         self._check_contains(v)
+        if self[v].kind in (OpKind.CACHE, OpKind.CACHE_WRITE):
+            raise ValueError("A cache is no output: cache_read gives its numbers")
         self.outputs.append(v)
 
     def output_all(self, values: Iterable[Value]):
@@ -945,6 +1099,11 @@ class Graph:
           SOFTMAX    u32 input, u32 axis
           LAYERNORM  u32 input, u32 axis, f32 eps
           REDUCE     u32 input, u8 op, u32 count, count x u32 axes
+          CACHE      u32 index
+          CACHE_WRITE      u32 cache, keys, values, start, count (0xffffffff: none, here and below)
+          CACHE_READ       u32 cache
+          CACHE_ATTENTION  u32 query, cache, start, count, slopes, prefix, prefix_length, f32 scale, f32 softcap, u32 window
+          SAMPLE           u32 logits, uniform, temperature, top_k, top_p, min_p
         """
         parts = []          # large constants are appended as they are (one copy, in the final join)
         out = bytearray()
@@ -1005,6 +1164,18 @@ class Graph:
                 out += struct.pack("<IBI", info.inputs[0], int(info.reduce_op), len(info.axes))
                 for a in info.axes:
                     out += struct.pack("<I", a)
+            elif k == OpKind.CACHE:
+                out += struct.pack("<I", info.input_index)
+            elif k == OpKind.CACHE_READ:
+                out += struct.pack("<I", info.inputs[0])
+            elif k in (OpKind.CACHE_WRITE, OpKind.CACHE_ATTENTION, OpKind.SAMPLE):
+                fixed = {OpKind.CACHE_WRITE: 4, OpKind.CACHE_ATTENTION: 3, OpKind.SAMPLE: 2}[k]
+                given, ids = iter(info.inputs[fixed:]), list(info.inputs[:fixed])
+                for there in info.present + ((info.present[2],) if k == OpKind.CACHE_ATTENTION else ()):   # (prefix_length with prefix)
+                    ids.append(next(given) if there else 0xFFFFFFFF)
+                out += struct.pack(f"<{len(ids)}I", *ids)
+                if k == OpKind.CACHE_ATTENTION:
+                    out += struct.pack("<ffI", *info.attention)
             else:
                 raise AssertionError(k)
         parts.append(bytes(out))

@@ -53,8 +53,13 @@ def optimize_graph(graph: Graph, settings: OptimizerSettings = OptimizerSettings
     for old in graph.inputs:
         info = graph[old]
         opt.map[old.index] = opt.new.input(info.shape, info.dtype)
+    for old in graph.caches:
+        opt.map[old.index] = opt.new._push_cache(graph[old])
     for old in graph.outputs:
         opt.new.output(opt.visit_completely(old))
+    for i, info in enumerate(graph.values):      # caches are written whether or not an output depends on it
+        if info.kind == OpKind.CACHE_WRITE:
+            opt.visit_completely(graph._v(i))
     return opt.new
 
 
@@ -64,6 +69,8 @@ def _clone(graph: Graph) -> Graph:
     for info in graph.values:
         if info.kind == OpKind.INPUT:
             new.input(info.shape, info.dtype)
+        elif info.kind == OpKind.CACHE:
+            new._push_cache(info)
         else:
             new._push(dataclasses.replace(info, non_output_uses=0))
     if len(new.values) != len(graph.values):

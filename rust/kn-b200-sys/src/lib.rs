@@ -67,6 +67,10 @@ pub struct kn_comm {
     _private: [u8; 0],
 }
 #[repr(C)]
+pub struct kn_cache {
+    _private: [u8; 0],
+}
+#[repr(C)]
 pub struct kn_outputs {
     _private: [u8; 0],
 }
@@ -115,6 +119,12 @@ extern "C" {
     pub fn kn_comm_create(device: c_int, rank: c_int, world: c_int, id: *const c_void, id_bytes: usize, out: *mut *mut kn_comm) -> c_int;
     pub fn kn_comm_destroy(comm: *mut kn_comm);
     pub fn kn_executor_set_comm(exec: *mut kn_executor, comm: *mut kn_comm) -> c_int;
+
+    pub fn kn_cache_create(device: c_int, sequences: usize, heads: usize, capacity: usize, dim: usize, dtype: c_int, out: *mut *mut kn_cache) -> c_int;
+    pub fn kn_cache_destroy(cache: *mut kn_cache);
+    pub fn kn_cache_bytes(cache: *const kn_cache, bytes: *mut u64) -> c_int;
+    pub fn kn_executor_cache_count(exec: *const kn_executor, n_caches: *mut c_int) -> c_int;
+    pub fn kn_executor_set_cache(exec: *mut kn_executor, index: c_int, cache: *mut kn_cache) -> c_int;
 
     pub fn kn_executor_selftest_wait_expiry(exec: *mut kn_executor, limit_us: u32) -> c_int;
 

@@ -27,7 +27,13 @@
 //!   15 Reduce     u32 input, u8 reduce tag, u32 count, count x u32 axis
 //! ```
 //! (Tag 16, AllReduce: u32 input, is an extension the reference's `Graph` cannot express; only graphs built
-//! for tensor-parallel execution contain it.)
+//! for tensor-parallel execution contain it.  So are 17 to 21, for decoders that answer token by token, in graphs that a host
+//! writes itself; 0xffffffff stands for an operand that is left out:
+//!   17 Cache           u32 index
+//!   18 CacheWrite      u32 cache, u32 keys, u32 values, u32 start, u32 count
+//!   19 CacheRead       u32 cache
+//!   20 CacheAttention  u32 query, cache, start, count, slopes, prefix, prefix_length, f32 scale, f32 softcap, u32 window
+//!   21 Sample          u32 logits, uniform, temperature, top_k, top_p, min_p)
 //!
 //! dtype tags are `DType`'s declaration order (kn-graph/src/dtype.rs:25-37); unary, binary and reduce tags are
 //! the declaration orders of `UnaryOp`, `BinaryOp`, `ReduceOp` (graph.rs:172-217).
@@ -53,6 +59,11 @@ pub const OP_BINARY: u8 = 12;
 pub const OP_SOFTMAX: u8 = 13;
 pub const OP_LAYERNORM: u8 = 14;
 pub const OP_REDUCE: u8 = 15;
+pub const OP_CACHE: u8 = 17;
+pub const OP_CACHE_WRITE: u8 = 18;
+pub const OP_CACHE_READ: u8 = 19;
+pub const OP_CACHE_ATTENTION: u8 = 20;
+pub const OP_SAMPLE: u8 = 21;
 
 pub const DTYPE_F32: u8 = 0;
 pub const DTYPE_F64: u8 = 1;
