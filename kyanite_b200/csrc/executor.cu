@@ -206,7 +206,6 @@ struct Executor {
         CacheParams c = planned;
         const auto& storage = caches[plan->buffers[t.buf].cache];
         c.base = storage ? storage->params.base : nullptr;
-        c.scales = storage ? storage->params.scales : nullptr;
         return c;
     }
 
@@ -1178,7 +1177,6 @@ int kn_cache_create(int device, size_t sequences, size_t heads, size_t capacity,
             cudaGetLastError();
             kn::fail(KN_ERR_CUDA, "no device memory for a cache of " + std::to_string(c->bytes) + " bytes: " + cudaGetErrorString(err));
         }
-        if (!c->params.half) c->params.scales = (float*)(c->params.base + kn::cache_rows(c->params) * c->params.row_bytes);
         KN_CUDA((cudaError_t)kn::cache_clear_async(c->params, nullptr));
         KN_CUDA(cudaStreamSynchronize(nullptr));
         *out = new kn_cache{std::move(c)};

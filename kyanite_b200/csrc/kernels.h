@@ -287,20 +287,17 @@ struct AllReduceParams {
     uint8_t dtype;     // DType: F32 or F16
 };
 
-// ---- the cache of a decoder: keys and values of every position of every sequence.  Storage (kn_cache_create): rows of `row_bytes`,
-// one per part (0 keys, 1 values), sequence, head and position, in that order, `padded` positions to a head; behind them, of an
-// i8 cache, their scales in the same order.  A row holds the channels, padded to a multiple of 64 with zeros, as f16 or as whole
-// numbers + 128, in 16-byte chunks whose order depends on the position (kernels/cache.cuh).
-constexpr int kCacheMaxDim = 256, kCachePositions = 64;   // capacities are padded to a multiple of these
+// ---- the cache of a decoder: keys and values of every position of every sequence.  Storage (kn_cache_create): tiles of 16 positions,
+// one per sequence, head and 16 positions, in that order.  A tile holds 16 rows of keys, 16 rows of values and, of an i8 cache, 16 scales
+// of keys and 16 of values; a row the channels, padded to a multiple of 64 with zeros, as f16 or as whole numbers + 128, in
+// 16-byte chunks whose order depends on the position (kernels/cache.cuh).
+constexpr int kCacheMaxDim = 256, kCacheTile = 16;
 struct CacheParams {
     uint8_t* base;
-    float* scales;           // null: f16
-    int64_t part_rows;       // rows between keys and values
-    int32_t seqs, heads, capacity, padded, dim, row_bytes, half;
+    int32_t seqs, heads, capacity, dim, tiles /* of a head */, tile_bytes, row_bytes, half;
 };
-int64_t cache_rows(const CacheParams& c);      // rows in all
 int64_t cache_bytes(const CacheParams& c);     // of all of it
-CacheParams cache_params(int64_t seqs, int64_t heads, int64_t capacity, int64_t dim, DType dtype);   // without pointers
+CacheParams cache_params(int64_t seqs, int64_t heads, int64_t capacity, int64_t dim, DType dtype);   // without the pointer
 int cache_clear_async(const CacheParams& c, cudaStream_t stream);   // all zeros
 
 // New tokens into the cache: token t of sequence s at position start[s] + t, the first count[s] of them

@@ -12,23 +12,22 @@
 
 namespace kn {
 
-int64_t cache_rows(const CacheParams& c) { return 2 * c.part_rows; }
-int64_t cache_bytes(const CacheParams& c) { return cache_rows(c) * (c.row_bytes + (c.half ? 0 : 4)); }
+int64_t cache_bytes(const CacheParams& c) { return (int64_t)c.seqs * c.heads * c.tiles * c.tile_bytes; }
 
 CacheParams cache_params(int64_t seqs, int64_t heads, int64_t capacity, int64_t dim, DType dtype) {
     CacheParams c{};
     c.half = dtype == DType::F16;
     c.seqs = (int32_t)seqs, c.heads = (int32_t)heads, c.capacity = (int32_t)capacity, c.dim = (int32_t)dim;
-    c.padded = (int32_t)((capacity + kCachePositions - 1) / kCachePositions * kCachePositions);
+    c.tiles = (int32_t)((capacity + kCacheTile - 1) / kCacheTile);
     c.row_bytes = (int32_t)((dim + 63) / 64 * 64) * (c.half ? 2 : 1);
-    c.part_rows = seqs * heads * c.padded;
+    c.tile_bytes = 2 * kCacheTile * c.row_bytes + (c.half ? 0 : 2 * kCacheTile * 4);
     return c;
 }
 
 int cache_clear_async(const CacheParams& c, cudaStream_t stream) {
-    const size_t rows = (size_t)cache_rows(c), bytes = rows * c.row_bytes;
+    const size_t rows = 2 * kCacheTile * (size_t)c.row_bytes, bytes = (size_t)cache_bytes(c);
     cudaError_t e = cudaMemsetAsync(c.base, c.half ? 0 : (int)(kCacheZeros & 0xff), bytes, stream);
-    if (e == cudaSuccess && !c.half) e = cudaMemsetAsync(c.scales, 0, rows * 4, stream);
+    if (e == cudaSuccess && !c.half) e = cudaMemset2DAsync(c.base + rows, (size_t)c.tile_bytes, 0, (size_t)c.tile_bytes - rows, bytes / c.tile_bytes, stream);
     return (int)e;
 }
 
@@ -82,8 +81,8 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant_
         const bool keep = live && position >= 0 && position < c.capacity && (p.count == nullptr || t < p.count[s]);
         const T* row = (const T*)p.in[part] + s * p.strides[part][0] + t * p.strides[part][1] + h * p.strides[part][2];
         const Eight e = load_eight<T, VEC>(row, p.strides[part][3], d, c.dim);
-        const int64_t to = cache_row(c, part, s, h, keep ? position : 0);
-        uint8_t* out = c.base + to * c.row_bytes;
+        const int64_t head = s * c.heads + h;
+        uint8_t* out = cache_row(c, part, head, keep ? (int)position : 0);
         if (c.half) {
             __half2 q[4];
 #pragma unroll
@@ -110,7 +109,7 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant_
             q[i >> 2] |= (uint32_t)((int)y + 128) << (8 * (i & 3));
         }
         if (keep && d < c.dim) *(uint2*)(out + (((d >> 4) ^ cache_swizzle(c.row_bytes, (int)position)) << 4) + (d & 8)) = make_uint2(q[0], q[1]);
-        if (keep && d == 0) c.scales[to] = scale;
+        if (keep && d == 0) *cache_scale(c, part, head, (int)position) = scale;
     }
 }
 
@@ -122,21 +121,22 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__
     const int d = (threadIdx.x % THREADS) * 8;
     if (d >= c.dim) return;
     const int t0 = blockIdx.x * kRows * kEach + threadIdx.x / THREADS;
-    const int64_t heads = 2ll * c.seqs * c.heads;
-    for (int64_t head = blockIdx.y; head < heads; head += gridDim.y) {
+    const int64_t heads = (int64_t)c.seqs * c.heads;
+    for (int64_t both = blockIdx.y; both < 2 * heads; both += gridDim.y) {   // part and head
+        const int part = both >= heads;
+        const int64_t head = both - part * heads;
         uint4 raw[kEach];
         float scale[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
             const int t = t0 + i * kRows;
-            const int64_t row = head * c.padded + min(t, c.capacity - 1);
-            const uint8_t* in = c.base + row * c.row_bytes;
-            const int x = cache_swizzle(c.row_bytes, min(t, c.capacity - 1));
+            const int from = min(t, c.capacity - 1), x = cache_swizzle(c.row_bytes, from);
+            const uint8_t* in = cache_row(c, part, head, from);
             if (c.half) {
                 raw[i] = *(const uint4*)(in + (((d >> 3) ^ x) << 4));
             } else {
                 *(uint2*)&raw[i] = *(const uint2*)(in + (((d >> 4) ^ x) << 4) + (d & 8));
-                scale[i] = c.scales[row];
+                scale[i] = *cache_scale(c, part, head, from);
             }
         }
 #pragma unroll
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__
 #pragma unroll
                 for (int k = 0; k < 8; k++) x[k] = (float)((int)q[k] - 128) * scale[i];
             }
-            T* out = (T*)p.out + (head * c.capacity + t) * c.dim + d;
+            T* out = (T*)p.out + (both * c.capacity + t) * c.dim + d;
             if constexpr (VEC && sizeof(T) == 2) {
                 __half2 y[4];
 #pragma unroll

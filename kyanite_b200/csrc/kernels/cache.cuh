@@ -1,8 +1,9 @@
-// How a cache's rows lie in memory (CacheParams).  A row is one position of one head: its channels, padded to a multiple of 64,
-// as f16 or as whole numbers + 128 (the low byte of 1024 + 128 + q in f16, whence two instructions make f16 of two of them).
+// How a cache lies in memory (CacheParams).  A row is one position of one head: its channels, padded to a multiple of 64, as f16
+// or as whole numbers + 128 (the low byte of 1024 + 128 + q in f16, whence two instructions make f16 of two of them).  Keys, values
+// and scales of 16 positions lie together, so that one bulk copy brings all that is needed of them.
 //
-// The 16-byte chunks of a row are written in an order that depends on the position, so that 16 rows copied to shared memory as
-// they lie are read without bank conflicts both as the matrix instructions read keys (8 positions x 64 bytes) and as they
+// The 16-byte chunks of a row are written in an order that depends on the position, so that a tile copied to shared memory as
+// it lies is read without bank conflicts both as the matrix instructions read keys (8 positions x 64 bytes) and as they
 // read values (4 positions, 4 apart or so, x 32 bytes): kernels/cache_attention.cu.
 #pragma once
 #include <cuda_fp16.h>
@@ -21,8 +22,15 @@ constexpr uint32_t kCacheZeros = 0x80808080u;   // four channels that are 0
 __host__ __device__ __forceinline__ int cache_swizzle(int row_bytes, int t) {
     return row_bytes % 128 == 0 ? (((t >> 2) & 3) << 1) ^ ((t & 1) << 2) : ((t >> 3) & 1) << 1;
 }
-__host__ __device__ __forceinline__ int64_t cache_row(const CacheParams& c, int part, int64_t seq, int64_t head, int64_t t) {
-    return part * c.part_rows + (seq * c.heads + head) * c.padded + t;
+// A row's first byte and its scale; part 0: keys, 1: values
+__host__ __device__ __forceinline__ uint8_t* cache_tile(const CacheParams& c, int64_t head /* of all sequences */, int t) {
+    return c.base + (head * c.tiles + (t >> 4)) * c.tile_bytes;
+}
+__host__ __device__ __forceinline__ uint8_t* cache_row(const CacheParams& c, int part, int64_t head, int t) {
+    return cache_tile(c, head, t) + (part * kCacheTile + (t & 15)) * c.row_bytes;
+}
+__host__ __device__ __forceinline__ float* cache_scale(const CacheParams& c, int part, int64_t head, int t) {
+    return (float*)(cache_tile(c, head, t) + 2 * kCacheTile * c.row_bytes) + part * kCacheTile + (t & 15);
 }
 
 }  // namespace kn

@@ -606,7 +606,7 @@ def test_cache_handles_are_checked():
             with pytest.raises(KnError, match="no cache"):
                 call()
         good = KvCache(0, 2, 2, 40, 64)
-        assert good.nbytes == 2 * 2 * 2 * 64 * (64 + 4)
+        assert good.nbytes == 2 * 2 * 2 * 48 * (64 + 4)        # (positions in sixteens, a scale each)
         for sizes in ((1, 2, 40, 64), (2, 1, 40, 64), (2, 2, 41, 64), (2, 2, 40, 63), (2, 2, 40, 64, F16)):
             with pytest.raises(KnError):
                 ex.set_cache(0, KvCache(0, *sizes))
