@@ -321,6 +321,9 @@ struct Executor {
                         p.arrived = (uint32_t*)ptr[at++];
                     }
                     p.status = status_dev;
+                    const int unit = p.half ? 8 : 4;   // elements of 16 bytes
+                    p.q_wide = p.q_strides[3] == 1 && p.cache.dim % unit == 0 && (uintptr_t)p.query % 16 == 0;
+                    for (int d = 0; d < 3; d++) p.q_wide = p.q_wide && p.q_strides[d] % unit == 0;
                     break;
                 }
                 case StepKind::Sample: {

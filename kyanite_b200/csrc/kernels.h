@@ -327,11 +327,13 @@ struct CacheAttentionParams {
     uint32_t* status;              // word that the kernel raises when a bounded wait expires
     float scale, softcap;
     int32_t window, tokens, heads, half;
+    int32_t q_wide;                // queries' channels can be read 16 bytes at a time
     int32_t grid;                  // CTAs (cache_attention_plan)
 };
 struct CacheAttentionPlan {
     int32_t grid;
     int64_t items, partial_floats;
+    double units;                  // of work, where every sequence is as long as the cache: below 2^31
 };
 CacheAttentionPlan cache_attention_plan(const CacheAttentionParams& p);
 

@@ -136,8 +136,9 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
     constexpr int kWarps = G::kWarps, kThreads = kWarps * 32, kStages = G::kStages, kE = G::kE, RB = G::kRowBytes, kDim = G::kDim;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) unsigned long long bars[kWarps * kStages];
-    __shared__ int64_t scan_sum[kWarps], scan_at;
-    __shared__ int scan_seq, abandon, is_last;
+    __shared__ int scan_sum[kWarps], scan_at, scan_seq, abandon, is_last;
+    __shared__ int64_t row_to[G::kRows];
+    __shared__ bool row_sees[G::kRows];
     __shared__ float row_most[kWarps][G::kRows], row_sum[kWarps][G::kRows], row_all[G::kRows];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     float* const join = (float*)(smem + kWarps * kStages * G::kStage);
@@ -145,7 +146,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
     const uint32_t ring_at = tcp::smem_u32(ring), bar_at = tcp::smem_u32(&bars[warp * kStages]);
     if (lane == 0)
         for (int i = 0; i < kStages; i++) tcp::mbar_init(bar_at + 8 * i, 1);
-    if (threadIdx.x == 0) abandon = 0, scan_seq = 0, scan_at = 0;
+    if (threadIdx.x == 0) abandon = 0, scan_seq = -1, scan_at = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     pdl_enter();
     const int group = p.heads / p.cache.heads, rows = group * p.tokens;
@@ -153,14 +154,16 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
     const int shared = p.prefix.base ? min(max(*p.prefix_length, 0), p.prefix.capacity) : 0;
     __syncthreads();
 
-    // ---- this CTA's range of the list: units [u0, u1), where u0 lies
+    // ---- what this CTA does: `todo` units from unit first_from of item first_item of sequence first_seq on
     const auto units_of = [&](const Span& z) { return max(1, (z.tiles + kWarps - 1) / kWarps); };
-    const auto scan = [&](int chunk, int64_t& mine) {   // sum over the sequences of a chunk up to and with this thread's
+    const auto units_at = [&](int s) { return units_of(span_of(p, s, shared)); };
+    // sum over the sequences of a chunk up to and with this thread's, of f(units of an item)
+    const auto scan = [&](int chunk, int& mine, auto f) {
         const int s = chunk * kThreads + threadIdx.x;
-        mine = s < p.cache.seqs ? (int64_t)units_of(span_of(p, s, shared)) * items : 0;
-        int64_t up = mine;
+        mine = s < p.cache.seqs ? f(units_at(s)) * items : 0;
+        int up = mine;
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t w = __shfl_up_sync(0xffffffffu, up, o);
+            const int w = __shfl_up_sync(0xffffffffu, up, o);
             if (lane >= o) up += w;
         }
         __syncthreads();
@@ -169,68 +172,108 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
         for (int w = 0; w < warp; w++) up += scan_sum[w];
         return up;
     };
-    const int chunks = (p.cache.seqs + kThreads - 1) / kThreads;
-    int64_t total = 0, mine = 0, upto = 0;
-    for (int i = 0; i < chunks; i++) {
-        upto = scan(i, mine);
-        for (int w = 0; w < kWarps; w++) total += scan_sum[w];
+    // the sequence in whose part of that sum `x` lies
+    const auto find = [&](int x, auto f) {
+        int front = 0;
+        for (int i = 0; i * kThreads < p.cache.seqs; i++) {
+            int mine;
+            const int at = front + scan(i, mine, f) - mine;
+            if (at <= x && x < at + mine) scan_seq = i * kThreads + threadIdx.x, scan_at = at;
+            for (int w = 0; w < kWarps; w++) front += scan_sum[w];
+        }
+        __syncthreads();
+    };
+    const auto all_of = [](int n) { return n; };
+    int total = 0;   // units
+    if (p.cache.seqs <= 64) {   // (every warp for itself)
+        int mine = (lane < p.cache.seqs ? units_at(lane) : 0) + (lane + 32 < p.cache.seqs ? units_at(lane + 32) : 0);
+        total = __reduce_add_sync(0xffffffffu, mine) * items;
+    } else {
+        for (int i = 0; i * kThreads < p.cache.seqs; i++) {
+            int mine;
+            scan(i, mine, all_of);
+            for (int w = 0; w < kWarps; w++) total += scan_sum[w];
+        }
     }
-    // (as many CTAs as there are units at most: each has some, and counts where an item's parts are joined)
-    const int64_t ctas = min((int64_t)gridDim.x, total), u0 = total * blockIdx.x / ctas, u1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : u0;
-    int64_t front = 0;
-    for (int i = 0; i < chunks; i++) {
-        if (chunks > 1) upto = scan(i, mine);
-        const int64_t at = front + upto - mine;
-        if (at <= u0 && u0 < at + mine) scan_seq = i * kThreads + threadIdx.x, scan_at = at;
-        for (int w = 0; w < kWarps; w++) front += scan_sum[w];
+    const int grid = gridDim.x;
+    // Items in whole parts of up to `most` units, one part per CTA, where that is hardly longer than equal ranges: a CTA does not change
+    // items then.  (A change and a join are about as long as two units.)
+    int most = 0;
+    if (p.cache.seqs <= 64) {
+        const int lane_units[2] = {lane < p.cache.seqs ? units_at(lane) : 0, lane + 32 < p.cache.seqs ? units_at(lane + 32) : 0};
+        const int least = (total + grid - 1) / grid;
+        for (int q = least; q <= least + 2 && most == 0; q++)
+            if (__reduce_add_sync(0xffffffffu, (lane_units[0] + q - 1) / q + (lane_units[1] + q - 1) / q) * items <= grid) most = q;
     }
-    __syncthreads();
-    if (u0 >= u1) return;
-    const int first_seq = scan_seq;
+    // in equal ranges the first `longer` CTAs have one unit more
+    const int ctas = min(grid, total), each = total / ctas, longer = total - each * ctas;
+    const auto cta_of = [&](int u) { return u < longer * (each + 1) ? u / (each + 1) : longer + (u - longer * (each + 1)) / each; };
+    const auto start_of = [&](int b) { return b * each + min(b, longer); };
+    int first_seq, first_item, first_from, todo, part = 0;
+    const int u0 = start_of(blockIdx.x);   // (equal ranges)
+    if (most > 0) {
+        find(blockIdx.x, [&](int n) { return (n + most - 1) / most; });
+        first_seq = scan_seq;
+        if (first_seq < 0) return;
+        const int units = units_at(first_seq), parts = (units + most - 1) / most, at = blockIdx.x - scan_at;
+        first_item = at / parts;
+        part = at % parts;
+        first_from = (int)((int64_t)units * part / parts);
+        todo = (int)((int64_t)units * (part + 1) / parts) - first_from;
+    } else {
+        if ((int)blockIdx.x >= ctas) return;
+        find(u0, all_of);
+        first_seq = scan_seq;
+        const int units = units_at(first_seq);
+        first_item = (u0 - scan_at) / units;
+        first_from = (u0 - scan_at) % units;
+        todo = each + ((int)blockIdx.x < longer ? 1 : 0);
+    }
     int issued = 0, consumed = 0;
 
     // ---- bulk copies of this warp's tiles, as far ahead as the ring goes: run after run, item after item
     Span next_span = span_of(p, first_seq, shared);
     int next_s = first_seq, next_units = units_of(next_span), next_run = -1, next_left = 0;
-    const int first_item = (int)((u0 - scan_at) / next_units), first_from = (int)((u0 - scan_at) % next_units);
-    int next_item = first_item, next_from = first_from;
-    int64_t next_u = u0;
+    int next_item = first_item, next_from = first_from, next_todo = todo, next_stage = 0;
     const uint8_t* next_tile = nullptr;
     const auto issue = [&]() {
         while (issued - consumed < kStages) {
             while (next_left == 0) {   // the next run that has a tile for this warp
                 if (next_run == 1) {
-                    next_u += next_units - next_from;
+                    next_todo -= next_units - next_from;
                     next_from = 0;
                     next_run = -1;
                     if (++next_item == items) {
                         next_item = 0;
-                        if (next_u < u1) {
+                        if (next_todo > 0) {
                             next_span = span_of(p, ++next_s, shared);
                             next_units = units_of(next_span);
                         }
                     }
                 }
-                if (next_u >= u1) return;
-                const int until = (int)min((int64_t)next_units, next_from + (u1 - next_u));
+                if (next_todo <= 0) return;
+                const int until = min(next_units, next_from + next_todo);
                 const Run r = run_of(next_span, ++next_run, next_from, until, warp, kWarps);
                 next_left = r.count;
                 const CacheParams& k = next_run ? p.cache : p.prefix;
                 next_tile = cache_tile(k, (next_run ? (int64_t)next_s * k.heads : 0) + next_item / row_tiles, r.first * kTile);
             }
-            const int stage = issued % kStages;
             if (tcp::elect_one()) {
-                tcp::mbar_expect_tx(bar_at + 8 * stage, G::kStage);
-                bulk_load(ring_at + stage * G::kStage, next_tile, G::kStage, bar_at + 8 * stage);
+                tcp::mbar_expect_tx(bar_at + 8 * next_stage, G::kStage);
+                bulk_load(ring_at + next_stage * G::kStage, next_tile, G::kStage, bar_at + 8 * next_stage);
             }
+            next_stage = next_stage + 1 == kStages ? 0 : next_stage + 1;
             next_tile += kWarps * G::kStage;
             next_left--;
             issued++;
         }
     };
     // (the same answer for all lanes, also where the wait runs out)
-    const auto wait_tile = [&]() {
-        return __all_sync(0xffffffffu, tcp::mbar_wait(bar_at + 8 * (consumed % kStages), (consumed / kStages) & 1, &abandon, p.status, kWaitCode));
+    int stage_at = 0, phase = 0;   // of the tile that is waited for
+    const auto wait_tile = [&]() { return __all_sync(0xffffffffu, tcp::mbar_wait(bar_at + 8 * stage_at, phase, &abandon, p.status, kWaitCode)); };
+    const auto done_tile = [&]() {
+        consumed++;
+        if (++stage_at == kStages) stage_at = 0, phase ^= 1;
     };
 
     // ---- where this lane's operands lie in a tile: keys at positions token[0] and token[1], a row of the first product each; values at
@@ -250,12 +293,12 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
 
     bool dead = false;
     Span span = next_span;
-    int64_t u = u0;
-    for (int seq = first_seq, item = first_item, first_unit = first_from; u < u1;) {
+    int u = u0;   // (equal ranges)
+    for (int seq = first_seq, item = first_item, first_unit = first_from; todo > 0;) {
         // ---- an item, or the part of it that is this CTA's: units [first_unit, until) of its own
         const int head = item / row_tiles, row0 = (item % row_tiles) * G::kRows;
         const int units = units_of(span);
-        const int until = (int)min((int64_t)units, first_unit + (u1 - u));
+        const int until = min(units, first_unit + todo);
         if (!dead) issue();
         // queries: row g of each eight
         uint32_t q[COLS][F32Q ? 2 : 1][G::kGroups][G::kSteps][2];
@@ -272,8 +315,16 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                 // brought near 2^14, so that the lower half keeps its bits in f16
                 const float* at = (const float*)p.query + from;
                 float most = 0.f;
-                if (has)
+                if (has && p.q_wide) {
+#pragma unroll
+                    for (int d = 4 * c; d < kDim; d += 16)
+                        if (d < p.cache.dim) {
+                            const float4 x = *(const float4*)(at + d);
+                            most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+                        }
+                } else if (has) {
                     for (int d = c; d < p.cache.dim; d += 4) most = fmaxf(most, fabsf(at[d * p.q_strides[3]]));
+                }
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
                 const int e = (__float_as_int(most) >> 23) - 127;   // (of an infinity 128: the row's result is NaN then)
@@ -283,25 +334,50 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
 #pragma unroll
             for (int k = 0; k < 2; k++) factor[n][k] = p.scale * (F32Q ? __int_as_float((127 - __shfl_sync(0xffffffffu, by, 4 * (2 * c + k))) << 23) : 1.f);
 #pragma unroll
-            for (int k = 0; k < G::kGroups; k++)
+            for (int k = 0; k < G::kGroups; k++) {
+                const int d0 = k * 4 * kN + c * kN;   // channels d0 to d0 + kN - 1 of the row
+                if constexpr (F32Q) {
+                    const float* at = (const float*)p.query + from;
+                    float x[kN];
 #pragma unroll
-                for (int st = 0; st < G::kSteps; st++)
+                    for (int i = 0; i < kN; i++) x[i] = 0.f;
+                    if (has && p.q_wide) {
 #pragma unroll
-                    for (int pair = 0; pair < 2; pair++) {
-                        const int d = k * 4 * kN + c * kN + 4 * st + 2 * pair;
-                        const bool one = has && d < p.cache.dim, two = has && d + 1 < p.cache.dim;
-                        if constexpr (F32Q) {
-                            const float* at = (const float*)p.query + from;
-                            const float x = one ? at[d * p.q_strides[3]] * amount : 0.f, y = two ? at[(d + 1) * p.q_strides[3]] * amount : 0.f;
-                            q[n][0][k][st][pair] = pack(x, y);
-                            const float2 back = unpack(q[n][0][k][st][pair]);
-                            q[n][F32Q ? 1 : 0][k][st][pair] = pack(x - back.x, y - back.y);
-                        } else {
-                            const __half* at = (const __half*)p.query + from;
-                            const __half2 both = __halves2half2(one ? at[d * p.q_strides[3]] : __half(0.f), two ? at[(d + 1) * p.q_strides[3]] : __half(0.f));
-                            q[n][0][k][st][pair] = *(const uint32_t*)&both;
-                        }
+                        for (int i = 0; i < kN; i += 4)
+                            if (d0 + i < p.cache.dim) *(float4*)(x + i) = *(const float4*)(at + d0 + i);
+                    } else if (has) {
+#pragma unroll
+                        for (int i = 0; i < kN; i++)
+                            if (d0 + i < p.cache.dim) x[i] = at[(d0 + i) * p.q_strides[3]];
                     }
+#pragma unroll
+                    for (int i = 0; i < kN; i += 2) {
+                        const uint32_t hi = pack(x[i] * amount, x[i + 1] * amount);
+                        const float2 back = unpack(hi);
+                        q[n][0][k][i >> 2][i >> 1 & 1] = hi;
+                        q[n][F32Q ? 1 : 0][k][i >> 2][i >> 1 & 1] = pack(x[i] * amount - back.x, x[i + 1] * amount - back.y);
+                    }
+                } else {
+                    const __half* at = (const __half*)p.query + from;
+                    uint32_t x[kN / 2];
+#pragma unroll
+                    for (int i = 0; i < kN / 2; i++) x[i] = 0;
+                    if (has && p.q_wide) {
+#pragma unroll
+                        for (int i = 0; i < kN / 2; i += 4)
+                            if (d0 + 2 * i < p.cache.dim) {
+                                const uint4 raw = *(const uint4*)(at + d0 + 2 * i);
+                                x[i] = raw.x, x[i + 1] = raw.y, x[i + 2] = raw.z, x[i + 3] = raw.w;
+                            }
+                    } else if (has) {
+#pragma unroll
+                        for (int i = 0; i < kN; i++)
+                            if (d0 + i < p.cache.dim) x[i >> 1] |= (uint32_t)__half_as_ushort(at[(d0 + i) * p.q_strides[3]]) << (16 * (i & 1));
+                    }
+#pragma unroll
+                    for (int i = 0; i < kN / 2; i++) q[n][0][k][i >> 1][i & 1] = x[i];
+                }
+            }
         }
         // this lane's columns
         float slope[COLS][2];
@@ -350,7 +426,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                     break;
                 }
                 const int at = tiles.first * kTile;
-                const uint8_t* stage = ring + (consumed % kStages) * G::kStage;
+                const uint8_t* stage = ring + stage_at * G::kStage;
                 if (t_first <= t_last) {   // (else rows of nothing but padding, of a sequence that has others)
                     // ---- scores: 16 positions x 8 rows
                     float s[COLS][4] = {};
@@ -570,7 +646,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                             }
                         }
                 }
-                consumed++;
+                done_tile();
                 __syncwarp();
                 issue();
             }
@@ -596,7 +672,12 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
             const float m = most_of(r);
             float all = 0.f;
             for (int w = 0; w < kWarps; w++) all += row_sum[w][r] * (m == -INFINITY ? 0.f : exp2_fast(row_most[w][r] - m));
-            row_all[r] = all;   // (read behind the next barrier)
+            // (read behind the next barrier)
+            row_all[r] = all;
+            const int row = row0 + r, t = row / group;
+            const int64_t pos = shared + span.start + t, last = min(pos, (int64_t)shared + p.cache.capacity - 1);
+            row_sees[r] = row < rows && t >= span.t_lo && t < span.t_hi && last >= 0 && (p.window == 0 || last > pos - p.window);
+            row_to[r] = (((int64_t)seq * p.tokens + t) * p.heads + head * group + row % group) * p.cache.dim;
         }
         float times[COLS][2];
 #pragma unroll
@@ -607,96 +688,107 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                 times[n][k] = m == -INFINITY ? 0.f : exp2_fast(ref[n][k] - m) * ((HALF ? 1.f : value_ref) / kWeight);
             }
         const bool whole = first_unit == 0 && until == units;
-        const int64_t slot = 2 * (int64_t)blockIdx.x + (u == u0 ? 0 : 1);
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (most > 0 || u == u0 ? 0 : 1);
         float* const partial = p.partial + slot * (G::kRows * (kDim + 2));
-        const auto visible = [&](int row) {   // does this row see anything
-            const int t = row / group;
-            if (row >= rows || t < span.t_lo || t >= span.t_hi) return false;
-            const int64_t pos = shared + span.start + t, last = min(pos, (int64_t)shared + p.cache.capacity - 1);
-            return last >= 0 && (p.window == 0 || last > pos - p.window);
+        const int rows_here = min(G::kRows, rows - row0);
+        const auto store = [&](int r, int d, float v) {
+            if (d >= p.cache.dim) return;
+            v = row_sees[r] ? v : 0.f;
+            if constexpr (F32Q) ((float*)p.out)[row_to[r] + d] = v;
+            else ((__half*)p.out)[row_to[r] + d] = __float2half_rn(v);
         };
-        const auto store = [&](int row, int d, float v) {
-            if (row >= rows || d >= p.cache.dim) return;
-            const int64_t to = (((int64_t)seq * p.tokens + row / group) * p.heads + head * group + row % group) * p.cache.dim + d;
-            if constexpr (F32Q) ((float*)p.out)[to] = v;
-            else ((__half*)p.out)[to] = __float2half_rn(v);
-        };
-        // four of a lane's channels of a block at a time: 32 of the block
+        // 32 of a block's channels (four of each lane's) of all rows, or more of them of fewer rows, at a time
+        constexpr int kPieces = G::kBlocks * kE / 4;
+        const int row_bits = rows_here <= 1 ? 0 : rows_here <= 2 ? 1 : rows_here <= 4 ? 2 : rows_here <= 8 ? 3 : 4;
+        const int at_once = G::kRows >> row_bits;   // pieces
 #pragma unroll
-        for (int b = 0; b < G::kBlocks; b++)
+        for (int piece = 0; piece < kPieces; piece++) {
+            const int b = piece / (kE / 4), i0 = piece % (kE / 4) * 2, place = piece & (at_once - 1);
 #pragma unroll
-            for (int i0 = 0; i0 < kE / 2; i0 += 2) {
+            for (int n = 0; n < COLS; n++)
 #pragma unroll
-                for (int n = 0; n < COLS; n++)
-#pragma unroll
-                    for (int k = 0; k < 2; k++)
-                        *(float4*)(join + (warp * G::kRows + 8 * n + 2 * c + k) * 32 + 4 * g) =
+                for (int k = 0; k < 2; k++)
+                    if (8 * n + 2 * c + k < rows_here)
+                        *(float4*)(join + (((warp * at_once + place) << row_bits) + 8 * n + 2 * c + k) * 32 + 4 * g) =
                             make_float4(o[n][b][i0][k] * times[n][k], o[n][b][i0][2 + k] * times[n][k], o[n][b][i0 + 1][k] * times[n][k], o[n][b][i0 + 1][2 + k] * times[n][k]);
-                __syncthreads();
-                for (int at = threadIdx.x; at < G::kRows * 32; at += kThreads) {
-                    const int r = at >> 5, d = b * 8 * kE + kE * ((at & 31) >> 2) + 2 * i0 + (at & 3);
-                    if (row0 + r >= rows) continue;
-                    float v = 0.f;
+            if (place != at_once - 1 && piece != kPieces - 1) continue;
+            __syncthreads();
+            const int from = piece - place;
+            for (int at = threadIdx.x; at < (((place + 1) << row_bits) << 5); at += kThreads) {
+                const int r = (at >> 5) & ((1 << row_bits) - 1), which = from + (at >> (5 + row_bits));
+                if (r >= rows_here) continue;
+                const int d = which / (kE / 4) * 8 * kE + kE * ((at & 31) >> 2) + which % (kE / 4) * 4 + (at & 3);
+                float v = 0.f;
 #pragma unroll
-                    for (int w = 0; w < kWarps; w++) v += join[(w * G::kRows + r) * 32 + (at & 31)];
-                    if (whole) store(row0 + r, d, visible(row0 + r) ? v / row_all[r] : 0.f);
-                    else partial[r * kDim + d] = v;
-                }
-                __syncthreads();
+                for (int w = 0; w < kWarps; w++) v += join[w * G::kRows * 32 + at];
+                if (whole) store(r, d, v / row_all[r]);
+                else partial[r * kDim + d] = v;
             }
+            __syncthreads();
+        }
         if (!whole) {
             if (threadIdx.x < G::kRows) {
                 partial[G::kRows * kDim + 2 * threadIdx.x] = most_of(threadIdx.x);
                 partial[G::kRows * kDim + 2 * threadIdx.x + 1] = row_all[threadIdx.x];
             }
-            // ---- whoever is last joins the item's parts
-            const int64_t item_u = u - first_unit;   // the item's first unit; CTA b has units from total b / ctas on
-            const int64_t c0 = ((item_u + 1) * ctas - 1) / total, c1 = ((item_u + units) * ctas - 1) / total;
+            // ---- whoever is last joins the item's parts: of CTAs c0 to c1, the first one's its second where it has something in front
+            const int item_u = u - first_unit;   // the item's first unit
+            int c0, parts;
+            bool second = false;
+            if (most > 0) {
+                parts = (units + most - 1) / most;
+                c0 = blockIdx.x - part;
+            } else {
+                c0 = cta_of(item_u);
+                parts = cta_of(item_u + units - 1) - c0 + 1;
+                second = start_of(c0) < item_u;
+            }
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
                 uint32_t* arrived = p.arrived + (int64_t)seq * items + item;
                 const uint32_t before = atomicAdd(arrived, 1u);
-                is_last = before == (uint32_t)(c1 - c0);
+                is_last = before == (uint32_t)(parts - 1);
                 if (is_last) *arrived = 0;
                 __threadfence();
             }
             __syncthreads();
             if (is_last) {
-                const auto part_of = [&](int64_t b) { return p.partial + (2 * b + (b == c0 && total * b / ctas < item_u ? 1 : 0)) * (G::kRows * (kDim + 2)); };
-                for (int at = threadIdx.x; at < G::kRows * kDim / 4; at += kThreads) {
+                constexpr int64_t kPart = G::kRows * (kDim + 2);
+                const float* const first = p.partial + (2 * (int64_t)c0 + (second ? 1 : 0)) * kPart;
+                const auto part_of = [&](int i) { return i == 0 ? first : p.partial + 2 * (int64_t)(c0 + i) * kPart; };
+                for (int at = threadIdx.x; at < rows_here * kDim / 4; at += kThreads) {
                     const int r = at / (kDim / 4), d = at % (kDim / 4) * 4;
-                    if (row0 + r >= rows) continue;
                     float m = -INFINITY, all = 0.f;
-                    for (int64_t b = c0; b <= c1; b++) m = fmaxf(m, __ldcg(part_of(b) + G::kRows * kDim + 2 * r));
+#pragma unroll 8
+                    for (int i = 0; i < parts; i++) m = fmaxf(m, __ldcg(part_of(i) + G::kRows * kDim + 2 * r));
                     float4 v = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-                    for (int64_t b = c0; b <= c1; b++) {
-                        const float* part = part_of(b);
-                        const float2 state = __ldcg((const float2*)(part + G::kRows * kDim + 2 * r));
-                        const float4 x = __ldcg((const float4*)(part + r * kDim + d));
+#pragma unroll 8
+                    for (int i = 0; i < parts; i++) {
+                        const float2 state = __ldcg((const float2*)(part_of(i) + G::kRows * kDim + 2 * r));
+                        const float4 x = __ldcg((const float4*)(part_of(i) + r * kDim + d));
                         const float f = m == -INFINITY ? 0.f : exp2_fast(state.x - m);
                         all += f * state.y;
                         v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
                     }
-                    const bool some = visible(row0 + r);
-                    store(row0 + r, d, some ? v.x / all : 0.f);
-                    store(row0 + r, d + 1, some ? v.y / all : 0.f);
-                    store(row0 + r, d + 2, some ? v.z / all : 0.f);
-                    store(row0 + r, d + 3, some ? v.w / all : 0.f);
+                    store(r, d, v.x / all);
+                    store(r, d + 1, v.y / all);
+                    store(r, d + 2, v.z / all);
+                    store(r, d + 3, v.w / all);
                 }
             }
             __syncthreads();
         }
         u += until - first_unit;
+        todo -= until - first_unit;
         first_unit = 0;
         if (++item == items) {
             item = 0;
-            if (u < u1) span = span_of(p, ++seq, shared);
+            if (todo > 0) span = span_of(p, ++seq, shared);
         }
     }
     // (given up: what is under way still writes to this CTA's shared memory)
-    for (; dead && consumed < issued; consumed++) wait_tile();
+    for (; dead && consumed < issued; done_tile()) wait_tile();
 }
 
 // f(Geo, kernel) of the variant that takes p
@@ -729,6 +821,7 @@ CacheAttentionPlan cache_attention_plan(const CacheAttentionParams& p) {
         plan.items = p.cache.seqs * p.cache.heads * ((rows + G::kRows - 1) / G::kRows);
         const int64_t tiles = (p.cache.capacity + kTile - 1) / kTile + (p.prefix.dim ? (p.prefix.capacity + kTile - 1) / kTile : 0);
         const double most = (double)plan.items * ((tiles + G::kWarps - 1) / G::kWarps);
+        plan.units = most;
         plan.grid = (int32_t)std::min<double>(148 * G::kPerSm, most);
         plan.partial_floats = 2ll * plan.grid * G::kRows * (G::kDim + 2);
     });

@@ -792,6 +792,7 @@ class Planner {
         if (out.ss.size() == 0) return out;
         KN_CHECK((int64_t)p.tokens * p.heads * p.cache.seqs < (1ll << 31), KN_ERR_UNSUPPORTED, "cache attention: too many rows");
         const CacheAttentionPlan plan = cache_attention_plan(p);
+        KN_CHECK(plan.units < 2e9, KN_ERR_UNSUPPORTED, "cache attention: too much work for one step");
         p.grid = plan.grid;
         if (plan.partial_floats) {
             add(alloc_shared({plan.partial_floats}, DType::F32, v), 1);
