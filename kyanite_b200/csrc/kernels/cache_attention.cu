@@ -25,12 +25,15 @@
 #include "launch.cuh"
 #include "tc_ptx.cuh"
 
+#include <type_traits>
+
 namespace kn {
 
 namespace {
 
 constexpr int kTile = kCacheTile;
 constexpr uint32_t kWaitCode = 71;
+constexpr float kBottom = -3.402823466e38f;   // a row's reference before it has seen a score
 constexpr float kAbove = 8.f;                 // of a score over its row's reference, as a power of two
 constexpr float kWeight = 128.f;              // what a weight of 1 is in f16: up to 2^15 with kAbove, down to 2^-21 with all its bits
 
@@ -404,7 +407,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
             for (int b = 0; b < G::kBlocks; b++)
 #pragma unroll
                 for (int i = 0; i < kE / 2; i++) o[n][b][i][0] = o[n][b][i][1] = o[n][b][i][2] = o[n][b][i][3] = 0.f;
-            ref[n][0] = ref[n][1] = -INFINITY;
+            ref[n][0] = ref[n][1] = kBottom;
             sum[n][0] = sum[n][1] = 0.f;
         }
         float value_ref = 0.f, weight_scale = HALF ? kWeight : 0.f;   // values' scales are counted in `value_ref`, a power of two above all
@@ -419,6 +422,231 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
             const auto high = [&](int t) { return cut(min(zero + t + 1, end)); };
             const auto low = [&](int t) { return p.window > 0 ? cut(zero + t - p.window + 1) : -(1 << 30); };
             const int all_hi = high(t_first), any_hi = high(t_last), all_lo = low(t_last), any_lo = low(t_first);
+            // one tile, with or without positions that some row does not see
+            const auto do_tile = [&](auto tag, int at, const uint8_t* stage) {
+                constexpr bool MASKED = decltype(tag)::value;
+                // ---- scores: 16 positions x 8 rows
+                float s[COLS][4] = {};
+#pragma unroll
+                for (int k = 0; k < G::kGroups; k++) {
+                    uint32_t w[2][4];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const uint4 raw = *(const uint4*)(stage + (RB % 128 == 0 ? (key_at[j] ^ ((k & 1) << 6)) + 128 * (k >> 1) : key_at[j] + 64 * k));
+                        w[j][0] = raw.x, w[j][1] = raw.y, w[j][2] = raw.z, w[j][3] = raw.w;
+                    }
+#pragma unroll
+                    for (int st = 0; st < G::kSteps; st++) {
+                        uint32_t a[4];
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            a[j] = HALF ? w[j][(2 * st) & 3] : two_of<0>(w[j][st]);
+                            a[2 + j] = HALF ? w[j][(2 * st + 1) & 3] : two_of<2>(w[j][st]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < COLS; n++)
+#pragma unroll
+                            for (int half = 0; half < (F32Q ? 2 : 1); half++) mma(s[n], a, q[n][half][k][st][0], q[n][half][k][st][1]);
+                    }
+                }
+                float key_scale[2] = {1.f, 1.f}, value_scale[2] = {1.f, 1.f};
+                if constexpr (!HALF) {
+                    const float* scales = (const float*)(stage + 2 * kTile * RB);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) key_scale[j] = scales[token[j]], value_scale[j] = scales[kTile + token[j]];
+                }
+                // s[n][2 j + k]: position token[j], row 2 c + k
+#pragma unroll
+                for (int n = 0; n < COLS; n++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[n][i] *= HALF ? factor[n][i & 1] : key_scale[i >> 1] * factor[n][i & 1];
+                if (capped) {
+                    // tanh(y) = 1 - 2 / (1 + e^(2y)): off by 2^-22 of the cap, which f32 results do not take
+#pragma unroll
+                    for (int n = 0; n < COLS; n++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            if constexpr (F32Q) s[n][i] = cap * tanhf(s[n][i]);
+                            else s[n][i] = cap - __fdividef(2.f * cap, 1.f + exp2_fast(fminf(s[n][i], 126.f)));
+                        }
+                }
+                if (p.slopes) {
+#pragma unroll
+                    for (int n = 0; n < COLS; n++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) s[n][i] -= slope[n][i & 1] * ((float)(zero + t_of[n][i & 1]) - (float)(at + token[i >> 1]));
+                }
+                bool hidden[COLS][4] = {};
+                if constexpr (MASKED) {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int key = at + token[j];
+#pragma unroll
+                        for (int n = 0; n < COLS; n++)
+#pragma unroll
+                            for (int k = 0; k < 2; k++) {
+                                hidden[n][2 * j + k] = key < low(t_of[n][k]) || key >= high(t_of[n][k]);
+                                if (hidden[n][2 * j + k]) s[n][2 * j + k] = -INFINITY;
+                            }
+                        if (!HALF && (key < any_lo || key >= any_hi)) value_scale[j] = 0.f;
+                    }
+                }
+                // ---- references: of the rows, and of the values' scales
+                bool moves = !HALF && fmaxf(value_scale[0], value_scale[1]) > value_ref;
+                float above[COLS][4];   // scores, from the reference on
+#pragma unroll
+                for (int n = 0; n < COLS; n++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        above[n][i] = __fsub_rn(s[n][i], ref[n][i & 1]);   // (0 for the highest itself, whose weight is 1 to the last bit)
+                        moves = moves || above[n][i] > kAbove;
+                    }
+                if (__any_sync(0xffffffffu, moves)) {
+                    const auto of_column = [](float v) {   // over the eight lanes of a column
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                        return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                    };
+                    float shrink = 1.f;
+                    if constexpr (!HALF) {
+                        const float top = of_column(fmaxf(value_scale[0], value_scale[1]));
+                        if (top > value_ref) {
+                            // (the next power of two, but none so small that its inverse times kWeight overflows)
+                            const float next = __int_as_float(min(max((__float_as_int(top) >> 23) + 1, 32), 254) << 23);
+                            shrink = value_ref > 0.f ? value_ref / next : 0.f;
+                            value_ref = next;
+                            weight_scale = kWeight / next;
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < COLS; n++) {
+                        float keep[2];
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const float top = fmaxf(ref[n][k], of_column(fmaxf(s[n][k], s[n][2 + k])));
+                            keep[k] = exp2_fast(ref[n][k] - top);
+                            ref[n][k] = top;
+                            above[n][k] = __fsub_rn(s[n][k], top);
+                            above[n][2 + k] = __fsub_rn(s[n][2 + k], top);
+                            sum[n][k] *= keep[k];
+                            keep[k] *= shrink;
+                        }
+#pragma unroll
+                        for (int b = 0; b < G::kBlocks; b++)
+#pragma unroll
+                            for (int i = 0; i < kE / 2; i++)
+#pragma unroll
+                                for (int x = 0; x < 4; x++) o[n][b][i][x] *= keep[x & 1];
+                    }
+                }
+                // ---- weights, in two halves, transposed: of row g, positions 2 c and 2 c + 1, 2 c + 8 and 2 c + 9 of the product
+                uint32_t weight[COLS][2][2];
+#pragma unroll
+                for (int n = 0; n < COLS; n++) {
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float e = exp2_fast(above[n][i]);
+                        sum[n][i & 1] += e;
+                        w[i] = e * (HALF ? kWeight : value_scale[i >> 1] * weight_scale);
+                        if (MASKED && hidden[n][i]) w[i] = 0.f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const uint32_t hi = pack(w[2 * j], w[2 * j + 1]);
+                        const float2 back = unpack(hi);
+                        weight[n][0][j] = transposed(hi);
+                        weight[n][1][j] = transposed(pack(w[2 * j] - back.x, w[2 * j + 1] - back.y));
+                    }
+                }
+                // ---- values^T . weights^T.  f32: the tile's products by themselves, then added (the matrix unit cuts off what it adds)
+                const auto times = [&](int b, int i, const uint32_t (&a)[4]) {
+#pragma unroll
+                    for (int n = 0; n < COLS; n++) {
+                        if constexpr (F32Q) {
+                            float part[4] = {};
+                            mma(part, a, weight[n][1][0], weight[n][1][1]);
+                            mma(part, a, weight[n][0][0], weight[n][0][1]);
+#pragma unroll
+                            for (int x = 0; x < 4; x++) o[n][b][i][x] += part[x];
+                        } else {
+                            mma(o[n][b][i], a, weight[n][1][0], weight[n][1][1]);
+                            mma(o[n][b][i], a, weight[n][0][0], weight[n][0][1]);
+                        }
+                    }
+                };
+                bool odd = false;
+#pragma unroll
+                for (int b = 0; b < G::kBlocks; b++) {
+                    constexpr int kWords = kE * (HALF ? 2 : 1) / 4;
+                    uint32_t w[4][kWords];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const uint8_t* from = stage + value_at[r] + b * 8 * kE * (HALF ? 2 : 1);
+                        if constexpr (kWords == 4) {
+                            const uint4 raw = *(const uint4*)from;
+                            w[r][0] = raw.x, w[r][1] = raw.y, w[r][2] = raw.z, w[r][3] = raw.w;
+                        } else {
+                            const uint2 raw = *(const uint2*)from;
+                            w[r][0] = raw.x, w[r][1] = raw.y;
+                        }
+                    }
+                    if constexpr (HALF) {
+                        if constexpr (MASKED) {
+                            // what nobody sees, and infinities and NaN (added row by row below), count as 0
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const bool seen = at + value_token[r] >= any_lo && at + value_token[r] < any_hi;
+#pragma unroll
+                                for (int x = 0; x < kWords; x++) {
+                                    const bool lo = (w[r][x] & 0x7c00u) == 0x7c00u, hi = (w[r][x] & 0x7c000000u) == 0x7c000000u;
+                                    odd = odd || (seen && (lo || hi));
+                                    w[r][x] = seen ? w[r][x] & (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0xffffu : 0xffffffffu) : 0u;
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < kWords; x++) {
+                            const uint32_t a[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
+                                                   __byte_perm(w[2][x], w[3][x], 0x5410), __byte_perm(w[2][x], w[3][x], 0x7632)};
+                            times(b, x, a);
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < kWords; x++) {
+                            const uint32_t lo01 = __byte_perm(w[0][x], w[1][x], 0x5140), lo23 = __byte_perm(w[2][x], w[3][x], 0x5140);
+                            const uint32_t hi01 = __byte_perm(w[0][x], w[1][x], 0x7362), hi23 = __byte_perm(w[2][x], w[3][x], 0x7362);
+                            const uint32_t a[4] = {two_of<0>(lo01), two_of<2>(lo01), two_of<0>(lo23), two_of<2>(lo23)};
+                            times(b, 2 * x, a);
+                            const uint32_t a2[4] = {two_of<0>(hi01), two_of<2>(hi01), two_of<0>(hi23), two_of<2>(hi23)};
+                            times(b, 2 * x + 1, a2);
+                        }
+                    }
+                }
+                if constexpr (HALF && MASKED)
+                    if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+                        for (int r = 0; r < 16; r++) {   // position token[r / 8] of lanes 4 (r % 8) and on
+                            const int key = at + __shfl_sync(0xffffffffu, r < 8 ? token[0] : token[1], 4 * (r & 7));
+                            if (key < any_lo || key >= any_hi) continue;
+#pragma unroll
+                            for (int n = 0; n < COLS; n++)
+#pragma unroll
+                                for (int k = 0; k < 2; k++) {
+                                    if (key < low(t_of[n][k]) || key >= high(t_of[n][k])) continue;
+                                    // (what the weight is does not matter: an infinity stays one)
+#pragma unroll
+                                    for (int b = 0; b < G::kBlocks; b++)
+#pragma unroll
+                                        for (int d = 0; d < kE; d++) {
+                                            const int chunk = g ^ cache_swizzle(RB, key);
+                                            const float v = __half2float(*(const __half*)(stage + (kTile + (key & 15)) * RB + b * 128 + (chunk << 4) + 2 * d));
+                                            if (!(fabsf(v) <= 65504.f)) o[n][b][d >> 1][2 * (d & 1) + k] += v;
+                                        }
+                                }
+                        }
+                    }
+            };
 #pragma unroll 1
             for (; tiles.count > 0; tiles.count--, tiles.first += kWarps) {
                 if (!wait_tile()) {
@@ -428,223 +656,8 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                 const int at = tiles.first * kTile;
                 const uint8_t* stage = ring + stage_at * G::kStage;
                 if (t_first <= t_last) {   // (else rows of nothing but padding, of a sequence that has others)
-                    // ---- scores: 16 positions x 8 rows
-                    float s[COLS][4] = {};
-#pragma unroll
-                    for (int k = 0; k < G::kGroups; k++) {
-                        uint32_t w[2][4];
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const uint4 raw = *(const uint4*)(stage + (RB % 128 == 0 ? (key_at[j] ^ ((k & 1) << 6)) + 128 * (k >> 1) : key_at[j] + 64 * k));
-                            w[j][0] = raw.x, w[j][1] = raw.y, w[j][2] = raw.z, w[j][3] = raw.w;
-                        }
-#pragma unroll
-                        for (int st = 0; st < G::kSteps; st++) {
-                            uint32_t a[4];
-#pragma unroll
-                            for (int j = 0; j < 2; j++) {
-                                a[j] = HALF ? w[j][(2 * st) & 3] : two_of<0>(w[j][st]);
-                                a[2 + j] = HALF ? w[j][(2 * st + 1) & 3] : two_of<2>(w[j][st]);
-                            }
-#pragma unroll
-                            for (int n = 0; n < COLS; n++)
-#pragma unroll
-                                for (int half = 0; half < (F32Q ? 2 : 1); half++) mma(s[n], a, q[n][half][k][st][0], q[n][half][k][st][1]);
-                        }
-                    }
-                    float key_scale[2] = {1.f, 1.f}, value_scale[2] = {1.f, 1.f};
-                    if constexpr (!HALF) {
-                        const float* scales = (const float*)(stage + 2 * kTile * RB);
-#pragma unroll
-                        for (int j = 0; j < 2; j++) key_scale[j] = scales[token[j]], value_scale[j] = scales[kTile + token[j]];
-                    }
-                    // s[n][2 j + k]: position token[j], row 2 c + k
-#pragma unroll
-                    for (int n = 0; n < COLS; n++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) s[n][i] *= HALF ? factor[n][i & 1] : key_scale[i >> 1] * factor[n][i & 1];
-                    if (capped) {
-                        // tanh(y) = 1 - 2 / (1 + e^(2y)): off by 2^-22 of the cap, which f32 results do not take
-#pragma unroll
-                        for (int n = 0; n < COLS; n++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                if constexpr (F32Q) s[n][i] = cap * tanhf(s[n][i]);
-                                else s[n][i] = cap - __fdividef(2.f * cap, 1.f + exp2_fast(fminf(s[n][i], 126.f)));
-                            }
-                    }
-                    if (p.slopes) {
-#pragma unroll
-                        for (int n = 0; n < COLS; n++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) s[n][i] -= slope[n][i & 1] * ((float)(zero + t_of[n][i & 1]) - (float)(at + token[i >> 1]));
-                    }
-                    const bool masked = at < all_lo || at + kTile > all_hi;
-                    bool hidden[COLS][4] = {};
-                    if (masked) {
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const int key = at + token[j];
-#pragma unroll
-                            for (int n = 0; n < COLS; n++)
-#pragma unroll
-                                for (int k = 0; k < 2; k++) {
-                                    hidden[n][2 * j + k] = key < low(t_of[n][k]) || key >= high(t_of[n][k]);
-                                    if (hidden[n][2 * j + k]) s[n][2 * j + k] = -INFINITY;
-                                }
-                            if (!HALF && (key < any_lo || key >= any_hi)) value_scale[j] = 0.f;
-                        }
-                    }
-                    // ---- references: of the rows, and of the values' scales
-                    bool moves = !HALF && fmaxf(value_scale[0], value_scale[1]) > value_ref;
-#pragma unroll
-                    for (int n = 0; n < COLS; n++)
-#pragma unroll
-                        for (int k = 0; k < 2; k++) moves = moves || fmaxf(s[n][k], s[n][2 + k]) > ref[n][k] + kAbove;
-                    if (__any_sync(0xffffffffu, moves)) {
-                        const auto of_column = [](float v) {   // over the eight lanes of a column
-                            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-                            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-                            return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-                        };
-                        float shrink = 1.f;
-                        if constexpr (!HALF) {
-                            const float top = of_column(fmaxf(value_scale[0], value_scale[1]));
-                            if (top > value_ref) {
-                                // (the next power of two, but none so small that its inverse times kWeight overflows)
-                                const float next = __int_as_float(min(max((__float_as_int(top) >> 23) + 1, 32), 254) << 23);
-                                shrink = value_ref > 0.f ? value_ref / next : 0.f;
-                                value_ref = next;
-                                weight_scale = kWeight / next;
-                            }
-                        }
-#pragma unroll
-                        for (int n = 0; n < COLS; n++) {
-                            float keep[2];
-#pragma unroll
-                            for (int k = 0; k < 2; k++) {
-                                const float top = fmaxf(ref[n][k], of_column(fmaxf(s[n][k], s[n][2 + k])));
-                                keep[k] = top == ref[n][k] ? 1.f : exp2_fast(ref[n][k] - top);
-                                ref[n][k] = top;
-                                sum[n][k] *= keep[k];
-                                keep[k] *= shrink;
-                            }
-#pragma unroll
-                            for (int b = 0; b < G::kBlocks; b++)
-#pragma unroll
-                                for (int i = 0; i < kE / 2; i++)
-#pragma unroll
-                                    for (int x = 0; x < 4; x++) o[n][b][i][x] *= keep[x & 1];
-                        }
-                    }
-                    // ---- weights, in two halves, transposed: of row g, positions 2 c and 2 c + 1, 2 c + 8 and 2 c + 9 of the product
-                    uint32_t weight[COLS][2][2];
-#pragma unroll
-                    for (int n = 0; n < COLS; n++) {
-                        float w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float base = ref[n][i & 1] == -INFINITY ? 0.f : ref[n][i & 1];
-                            const float e = exp2_fast(s[n][i] - base);
-                            sum[n][i & 1] += e;
-                            w[i] = e * (HALF ? kWeight : value_scale[i >> 1] * weight_scale);
-                            if (masked && hidden[n][i]) w[i] = 0.f;
-                        }
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const uint32_t hi = pack(w[2 * j], w[2 * j + 1]);
-                            const float2 back = unpack(hi);
-                            weight[n][0][j] = transposed(hi);
-                            weight[n][1][j] = transposed(pack(w[2 * j] - back.x, w[2 * j + 1] - back.y));
-                        }
-                    }
-                    // ---- values^T . weights^T.  f32: the tile's products by themselves, then added (the matrix unit cuts off what it adds)
-                    const auto times = [&](int b, int i, const uint32_t (&a)[4]) {
-#pragma unroll
-                        for (int n = 0; n < COLS; n++) {
-                            if constexpr (F32Q) {
-                                float part[4] = {};
-                                mma(part, a, weight[n][1][0], weight[n][1][1]);
-                                mma(part, a, weight[n][0][0], weight[n][0][1]);
-#pragma unroll
-                                for (int x = 0; x < 4; x++) o[n][b][i][x] += part[x];
-                            } else {
-                                mma(o[n][b][i], a, weight[n][1][0], weight[n][1][1]);
-                                mma(o[n][b][i], a, weight[n][0][0], weight[n][0][1]);
-                            }
-                        }
-                    };
-                    bool odd = false;
-#pragma unroll
-                    for (int b = 0; b < G::kBlocks; b++) {
-                        constexpr int kWords = kE * (HALF ? 2 : 1) / 4;
-                        uint32_t w[4][kWords];
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const uint8_t* from = stage + value_at[r] + b * 8 * kE * (HALF ? 2 : 1);
-                            if constexpr (kWords == 4) {
-                                const uint4 raw = *(const uint4*)from;
-                                w[r][0] = raw.x, w[r][1] = raw.y, w[r][2] = raw.z, w[r][3] = raw.w;
-                            } else {
-                                const uint2 raw = *(const uint2*)from;
-                                w[r][0] = raw.x, w[r][1] = raw.y;
-                            }
-                        }
-                        if constexpr (HALF) {
-                            if (masked) {
-                                // what nobody sees, and infinities and NaN (added row by row below), count as 0
-#pragma unroll
-                                for (int r = 0; r < 4; r++) {
-                                    const bool seen = at + value_token[r] >= any_lo && at + value_token[r] < any_hi;
-#pragma unroll
-                                    for (int x = 0; x < kWords; x++) {
-                                        const bool lo = (w[r][x] & 0x7c00u) == 0x7c00u, hi = (w[r][x] & 0x7c000000u) == 0x7c000000u;
-                                        odd = odd || (seen && (lo || hi));
-                                        w[r][x] = seen ? w[r][x] & (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0xffffu : 0xffffffffu) : 0u;
-                                    }
-                                }
-                            }
-#pragma unroll
-                            for (int x = 0; x < kWords; x++) {
-                                const uint32_t a[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
-                                                       __byte_perm(w[2][x], w[3][x], 0x5410), __byte_perm(w[2][x], w[3][x], 0x7632)};
-                                times(b, x, a);
-                            }
-                        } else {
-#pragma unroll
-                            for (int x = 0; x < kWords; x++) {
-                                const uint32_t lo01 = __byte_perm(w[0][x], w[1][x], 0x5140), lo23 = __byte_perm(w[2][x], w[3][x], 0x5140);
-                                const uint32_t hi01 = __byte_perm(w[0][x], w[1][x], 0x7362), hi23 = __byte_perm(w[2][x], w[3][x], 0x7362);
-                                const uint32_t a[4] = {two_of<0>(lo01), two_of<2>(lo01), two_of<0>(lo23), two_of<2>(lo23)};
-                                times(b, 2 * x, a);
-                                const uint32_t a2[4] = {two_of<0>(hi01), two_of<2>(hi01), two_of<0>(hi23), two_of<2>(hi23)};
-                                times(b, 2 * x + 1, a2);
-                            }
-                        }
-                    }
-                    if constexpr (HALF)
-                        if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll 1
-                            for (int r = 0; r < 16; r++) {   // position token[r / 8] of lanes 4 (r % 8) and on
-                                const int key = at + __shfl_sync(0xffffffffu, r < 8 ? token[0] : token[1], 4 * (r & 7));
-                                if (key < any_lo || key >= any_hi) continue;
-#pragma unroll
-                                for (int n = 0; n < COLS; n++)
-#pragma unroll
-                                    for (int k = 0; k < 2; k++) {
-                                        if (key < low(t_of[n][k]) || key >= high(t_of[n][k])) continue;
-                                        // (what the weight is does not matter: an infinity stays one)
-#pragma unroll
-                                        for (int b = 0; b < G::kBlocks; b++)
-#pragma unroll
-                                            for (int d = 0; d < kE; d++) {
-                                                const int chunk = g ^ cache_swizzle(RB, key);
-                                                const float v = __half2float(*(const __half*)(stage + (kTile + (key & 15)) * RB + b * 128 + (chunk << 4) + 2 * d));
-                                                if (!(fabsf(v) <= 65504.f)) o[n][b][d >> 1][2 * (d & 1) + k] += v;
-                                            }
-                                    }
-                            }
-                        }
+                    if (at < all_lo || at + kTile > all_hi) do_tile(std::true_type{}, at, stage);
+                    else do_tile(std::false_type{}, at, stage);
                 }
                 done_tile();
                 __syncwarp();
@@ -671,7 +684,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
             const int r = threadIdx.x;
             const float m = most_of(r);
             float all = 0.f;
-            for (int w = 0; w < kWarps; w++) all += row_sum[w][r] * (m == -INFINITY ? 0.f : exp2_fast(row_most[w][r] - m));
+            for (int w = 0; w < kWarps; w++) all += row_sum[w][r] * exp2_fast(row_most[w][r] - m);
             // (read behind the next barrier)
             row_all[r] = all;
             const int row = row0 + r, t = row / group;
@@ -685,7 +698,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const float m = most_of(8 * n + 2 * c + k);
-                times[n][k] = m == -INFINITY ? 0.f : exp2_fast(ref[n][k] - m) * ((HALF ? 1.f : value_ref) / kWeight);
+                times[n][k] = exp2_fast(ref[n][k] - m) * ((HALF ? 1.f : value_ref) / kWeight);
             }
         const bool whole = first_unit == 0 && until == units;
         const int64_t slot = 2 * (int64_t)blockIdx.x + (most > 0 || u == u0 ? 0 : 1);
@@ -759,7 +772,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                 const auto part_of = [&](int i) { return i == 0 ? first : p.partial + 2 * (int64_t)(c0 + i) * kPart; };
                 for (int at = threadIdx.x; at < rows_here * kDim / 4; at += kThreads) {
                     const int r = at / (kDim / 4), d = at % (kDim / 4) * 4;
-                    float m = -INFINITY, all = 0.f;
+                    float m = kBottom, all = 0.f;
 #pragma unroll 8
                     for (int i = 0; i < parts; i++) m = fmaxf(m, __ldcg(part_of(i) + G::kRows * kDim + 2 * r));
                     float4 v = make_float4(0, 0, 0, 0);
@@ -767,7 +780,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                     for (int i = 0; i < parts; i++) {
                         const float2 state = __ldcg((const float2*)(part_of(i) + G::kRows * kDim + 2 * r));
                         const float4 x = __ldcg((const float4*)(part_of(i) + r * kDim + d));
-                        const float f = m == -INFINITY ? 0.f : exp2_fast(state.x - m);
+                        const float f = exp2_fast(state.x - m);
                         all += f * state.y;
                         v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
                     }
