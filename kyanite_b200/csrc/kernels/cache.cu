@@ -60,56 +60,98 @@ __device__ __forceinline__ Eight load_eight(const T* row, int64_t stride, int d,
     return e;
 }
 
-// THREADS threads a row (8 channels each).  VEC: rows whose channels are contiguous, 16-byte aligned and a multiple of 8
+// Four numbers + 128 in a word: round(x / scale), of the quotient that IEEE division gives.  With r = 1 / scale rounded to nearest, y = x r
+// and y + r (x - y scale), both in one rounding, is that quotient (Markstein 1990; scales next to either end of the range, and the one
+// mantissa of all ones, for which r may be off, divide).  Adding 1.5 x 2^23 rounds it half to even and leaves it in the low byte.
+__device__ __forceinline__ uint32_t low_bytes(const float (&y)[4]) {
+    uint32_t b[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) b[k] = __float_as_uint(__fadd_rn(y[k], 12582912.f + 128.f));
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint32_t four_of(const float* x, float scale, float r) {
+    float y[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        y[k] = x[k] * r;
+        y[k] = fmaf(fmaf(-y[k], scale, x[k]), r, y[k]);
+    }
+    return low_bytes(y);
+}
+// Rows for which that does not hold: the scale and eight numbers.  (A scale of few bits, of numbers next to nothing, may give more than 127)
+__device__ __noinline__ uint2 divided(const float* x, float most, float* scale) {
+    *scale = most < __int_as_float(0x7f800000) ? __fdiv_rn(most, 127.f) : __int_as_float(0x7fc00000);
+    float y[8];
+#pragma unroll 1
+    for (int k = 0; k < 8; k++) y[k] = *scale > 0.f ? fminf(fmaxf(__fdiv_rn(x[k], *scale), -127.f), 127.f) : 0.f;
+    const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
+    return make_uint2(low_bytes(lo), low_bytes(hi));
+}
+
+// THREADS threads a row (8 channels each), kEach rows a thread with their loads in flight together.  VEC: rows whose channels are
+// contiguous, 16-byte aligned and a multiple of 8.  A block takes positions of one head (and writes whole tiles), of few tokens heads of one
+// position (and reads what lies together).  7 prompts of up to 1500 tokens, 32 heads of 128 channels, f32 into i8 (270 MB): bound by
+// instructions while every row found its place by divisions and every number was divided: 149 us.
 template <typename T, bool VEC, int THREADS>
 __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant__ CacheWriteParams p) {
     pdl_enter();
+    constexpr int kRows = 256 / THREADS, kEach = 4;
     const CacheParams& c = p.cache;
     const int d = (threadIdx.x % THREADS) * 8;
-    const int64_t per_part = (int64_t)c.seqs * p.tokens * c.heads;
-    const int64_t rows = 2 * per_part, step = (int64_t)gridDim.x * (256 / THREADS);
-    // (all threads of a row go round as often as each other: they exchange the maximum)
-    for (int64_t r = (int64_t)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS; r - threadIdx.x / THREADS < rows; r += step) {
-        const bool live = r < rows;
-        const int64_t at = live ? r : rows - 1;
-        const int part = at >= per_part;
-        const int64_t token = (at - part * per_part) / c.heads;
-        const int h = (int)((at - part * per_part) - token * c.heads);
-        const int64_t s = token / p.tokens;
-        const int t = (int)(token - s * p.tokens);
-        const int64_t position = (int64_t)p.start[s] + t;
-        const bool keep = live && position >= 0 && position < c.capacity && (p.count == nullptr || t < p.count[s]);
-        const T* row = (const T*)p.in[part] + s * p.strides[part][0] + t * p.strides[part][1] + h * p.strides[part][2];
-        const Eight e = load_eight<T, VEC>(row, p.strides[part][3], d, c.dim);
-        const int64_t head = s * c.heads + h;
-        uint8_t* out = cache_row(c, part, head, keep ? (int)position : 0);
-        if (c.half) {
-            __half2 q[4];
+    const bool along = p.tokens >= 16;   // along the positions
+    const int inner = along ? p.tokens : c.heads, outer = along ? c.heads : p.tokens;
+    const int first = blockIdx.x * (kRows * kEach) + threadIdx.x / THREADS;
+    for (int y = blockIdx.y; y < 2 * c.seqs * outer; y += gridDim.y) {
+        const int part = y >= c.seqs * outer, rest = y - part * c.seqs * outer, s = rest / outer, fixed = rest - s * outer;
+        const int64_t start = p.start[s];
+        const int count = p.count != nullptr ? p.count[s] : p.tokens;
+        const T* in = (const T*)p.in[part] + s * p.strides[part][0] + fixed * p.strides[part][along ? 2 : 1];
+        const int64_t stride = p.strides[part][along ? 1 : 2], head_bytes = (int64_t)c.tiles * c.tile_bytes;
+        uint8_t* const tiles = c.base + ((int64_t)s * c.heads + (along ? fixed : 0)) * head_bytes;
+        Eight e[kEach];
+        int position[kEach];   // -1: not written
 #pragma unroll
-            for (int i = 0; i < 4; i++) q[i] = __floats2half2_rn(e.x[2 * i], e.x[2 * i + 1]);
-            if (keep && d < c.dim) *(uint4*)(out + (((d >> 3) ^ cache_swizzle(c.row_bytes, (int)position)) << 4)) = *(uint4*)q;
-            continue;
+        for (int i = 0; i < kEach; i++) {
+            const int r = first + i * kRows, t = along ? r : fixed;
+            const int64_t at = start + t;
+            position[i] = r < inner && t < count && at >= 0 && at < c.capacity ? (int)at : -1;
+            e[i] = position[i] >= 0 ? load_eight<T, VEC>(in + r * stride, p.strides[part][3], d, c.dim) : Eight{};
         }
-        float most = 0.f;
-        bool nan = false;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            most = fmaxf(most, fabsf(e.x[i]));
-            nan = nan || e.x[i] != e.x[i];
+        for (int i = 0; i < kEach; i++) {
+            if (!__any_sync(0xffffffffu, position[i] >= 0)) continue;
+            const int t = max(position[i], 0), x = cache_swizzle(c.row_bytes, t);
+            uint8_t* const tile = tiles + (along ? 0 : (first + i * kRows) * head_bytes) + (int64_t)(t >> 4) * c.tile_bytes;
+            uint8_t* const out = tile + (part * kCacheTile + (t & 15)) * c.row_bytes;
+            const bool keep = position[i] >= 0 && d < c.dim;
+            if (c.half) {
+                __half2 q[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) q[k] = __floats2half2_rn(e[i].x[2 * k], e[i].x[2 * k + 1]);
+                if (keep) *(uint4*)(out + (((d >> 3) ^ x) << 4)) = *(uint4*)q;
+                continue;
+            }
+            uint32_t most = 0;   // the largest magnitude as bits, a NaN above all others
+#pragma unroll
+            for (int k = 0; k < 8; k++) most = max(most, __float_as_uint(e[i].x[k]) & 0x7fffffffu);
+#pragma unroll
+            for (int o = THREADS / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const float top = __uint_as_float(most);
+            float scale = top * (1.f / 127.f);
+            scale = fmaf(fmaf(-scale, 127.f, top), 1.f / 127.f, scale);   // (top / 127, by the same argument)
+            uint2 q;
+            if (!(top > 1e-28f && top < 1e30f) || (__float_as_uint(scale) & 0x7fffffu) == 0x7fffffu) {
+                float y[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) y[k] = e[i].x[k];
+                q = divided(y, top, &scale);
+            } else {
+                const float inverse = __frcp_rn(scale);
+                q = make_uint2(four_of(e[i].x, scale, inverse), four_of(e[i].x + 4, scale, inverse));
+            }
+            if (keep) *(uint2*)(out + (((d >> 4) ^ x) << 4) + (d & 8)) = q;
+            if (keep && d == 0) ((float*)(tile + 2 * kCacheTile * c.row_bytes))[part * kCacheTile + (t & 15)] = scale;
         }
-        if (nan) most = __int_as_float(0x7f800000);
-#pragma unroll
-        for (int o = THREADS / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        const float scale = most < __int_as_float(0x7f800000) ? __fdiv_rn(most, 127.f) : __int_as_float(0x7fc00000);
-        uint32_t q[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            // (a scale of few bits, of numbers next to nothing, may give more than 127)
-            const float y = scale > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(e.x[i], scale)), -127.f), 127.f) : 0.f;
-            q[i >> 2] |= (uint32_t)((int)y + 128) << (8 * (i & 3));
-        }
-        if (keep && d < c.dim) *(uint2*)(out + (((d >> 4) ^ cache_swizzle(c.row_bytes, (int)position)) << 4) + (d & 8)) = make_uint2(q[0], q[1]);
-        if (keep && d == 0) *cache_scale(c, part, head, (int)position) = scale;
     }
 }
 
@@ -125,18 +167,20 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__
     for (int64_t both = blockIdx.y; both < 2 * heads; both += gridDim.y) {   // part and head
         const int part = both >= heads;
         const int64_t head = both - part * heads;
+        const uint8_t* const tiles = c.base + head * ((int64_t)c.tiles * c.tile_bytes);
+        T* const rows = (T*)p.out + both * c.capacity * c.dim + d;
         uint4 raw[kEach];
         float scale[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            const int t = t0 + i * kRows;
-            const int from = min(t, c.capacity - 1), x = cache_swizzle(c.row_bytes, from);
-            const uint8_t* in = cache_row(c, part, head, from);
+            const int t = min(t0 + i * kRows, c.capacity - 1), x = cache_swizzle(c.row_bytes, t);
+            const uint8_t* const tile = tiles + (int64_t)(t >> 4) * c.tile_bytes;
+            const uint8_t* const in = tile + (part * kCacheTile + (t & 15)) * c.row_bytes;
             if (c.half) {
                 raw[i] = *(const uint4*)(in + (((d >> 3) ^ x) << 4));
             } else {
                 *(uint2*)&raw[i] = *(const uint2*)(in + (((d >> 4) ^ x) << 4) + (d & 8));
-                scale[i] = *cache_scale(c, part, head, from);
+                scale[i] = ((const float*)(tile + 2 * kCacheTile * c.row_bytes))[part * kCacheTile + (t & 15)];
             }
         }
 #pragma unroll
@@ -145,15 +189,19 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__
             if (t >= c.capacity) break;
             float x[8];
             if (c.half) {
-                const __half* h = (const __half*)&raw[i];
+                const __half2* h = (const __half2*)&raw[i];
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[k] = __half2float(h[k]);
+                for (int k = 0; k < 4; k++) {
+                    const float2 f = __half22float2(h[k]);
+                    x[2 * k] = f.x, x[2 * k + 1] = f.y;
+                }
             } else {
-                const uint8_t* q = (const uint8_t*)&raw[i];
+                const uint32_t* q = (const uint32_t*)&raw[i];
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[k] = (float)((int)q[k] - 128) * scale[i];
+                for (int k = 0; k < 8; k++)   // 2^23 + byte, as it is in f32
+                    x[k] = (__uint_as_float(__byte_perm(q[k >> 2], 0x4b000000u, 0x7440 + (k & 3))) - (8388608.f + 128.f)) * scale[i];
             }
-            T* out = (T*)p.out + (both * c.capacity + t) * c.dim + d;
+            T* const out = rows + (int64_t)t * c.dim;
             if constexpr (VEC && sizeof(T) == 2) {
                 __half2 y[4];
 #pragma unroll
@@ -174,8 +222,10 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__
 template <typename T, bool VEC>
 void write_threads(const CacheWriteParams& p, cudaStream_t stream) {
     const int threads = p.cache.dim <= 64 ? 8 : p.cache.dim <= 128 ? 16 : 32;
-    const int64_t rows = 2ll * p.cache.seqs * p.tokens * p.cache.heads, per_block = 256 / threads;
-    const dim3 grid((unsigned)std::min<int64_t>((rows + per_block - 1) / per_block, 148 * 16));
+    const bool along = p.tokens >= 16;
+    const int per_block = 4 * 256 / threads, inner = along ? p.tokens : p.cache.heads;
+    const int64_t outer = 2ll * p.cache.seqs * (along ? p.cache.heads : p.tokens);
+    const dim3 grid((unsigned)((inner + per_block - 1) / per_block), (unsigned)std::min<int64_t>(outer, 65535));
     if (threads == 8) launch_pdl(cache_write_kernel<T, VEC, 8>, grid, dim3(256), 0, stream, p);
     if (threads == 16) launch_pdl(cache_write_kernel<T, VEC, 16>, grid, dim3(256), 0, stream, p);
     if (threads == 32) launch_pdl(cache_write_kernel<T, VEC, 32>, grid, dim3(256), 0, stream, p);

@@ -731,6 +731,7 @@ class Planner {
         s.desc = "cachewrite seqs=" + std::to_string(p.cache.seqs) + " tokens=" + std::to_string(p.tokens) + " heads=" + std::to_string(p.cache.heads) + " dim=" +
                  std::to_string(p.cache.dim) + (p.half ? " f16" : " f32") + " into " + dtype_name(info.dtype);
         if ((int64_t)p.tokens * p.cache.seqs == 0) return cache;
+        KN_CHECK(2.0 * p.tokens * p.cache.seqs * p.cache.heads < 2e9, KN_ERR_UNSUPPORTED, "cache write: too many rows for one step");
         const double row = p.cache.dim * (p.cache.half ? 2.0 : 1.0) + (p.cache.half ? 0 : 4);
         push_step(std::move(s));
         Step& pushed = plan_.steps.back();
