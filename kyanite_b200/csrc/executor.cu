@@ -332,6 +332,7 @@ struct Executor {
                     p.logits = ptr[0];
                     p.out = (int32_t*)ptr[1];
                     p.uniform = (const float*)ptr[2];
+                    p.status = status_dev;
                     size_t at = 3;
                     if (has.temperature) p.temperature = (const float*)ptr[at++];
                     if (has.top_k) p.top_k = (const int32_t*)ptr[at++];

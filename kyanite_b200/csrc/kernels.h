@@ -346,6 +346,7 @@ struct SampleParams {
     int32_t* out;
     int64_t rows, row_stride, col_stride;
     int32_t vocab, half;
+    uint32_t* status;              // word that the kernel raises when a bounded wait expires
 };
 
 // ---- small transfers between device memory and pinned host memory (kernels/host_copy.cu)

@@ -5,14 +5,20 @@
 // each is a cut: a key (the logit's bits in the order of whole numbers) and, among equal keys, an index.  A cut is found by
 // eight bits of the key at a time, from counts or weights per value of them.
 //
-// One CTA a row.
+// A row is read once, into the shared memory of a cluster of up to eight CTAs that share it.  Cuts are found from counts or weights of 1024
+// bins of the logits; a bin's tokens, if there are not too many, go to one CTA that ranks them all at once.  Weights are
+// computed in f64 by a table of 256 powers and four terms of a series: ten operations, where the general exp has some thirty.
+// Rows that do not fit, or whose tokens do not lie together, are read again and again by one CTA.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "../kernels.h"
 #include "launch.cuh"
+#include "tc_ptx.cuh"
 
 namespace kn {
 
@@ -208,9 +214,443 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     }
 }
 
+// ---- the usual rows: a cluster a row
+
+constexpr int kCta = 512, kWarps = kCta / 32, kPieces = 8;   // a warp's part of a row is summed in eight pieces
+constexpr int kBins = 1024, kList = 1024, kTable = 256;
+constexpr int kMaxCluster = 8;
+constexpr float kDepth = 32.f;   // weights below e^-32 count as 0 (2^-46 and less, in steps of 2^-44)
+
+// A number of some tokens and their weight
+struct Amount {
+    u64 mass;
+    uint32_t count;
+};
+
+// What the CTAs of a cluster tell each other, and what they share inside
+struct ClusterShared {
+    u64 bar;
+    u64 slots[2][kMaxCluster];            // from each CTA, two exchanges in turn
+    double table[kTable];                 // 2^44 2^(-k / 256)
+    u64 pieces[kWarps * kPieces], scan[kWarps];
+    uint32_t counts[kBins], limbs[3][kBins];   // weights of a bin in 15, 15 and 14 bits: no sum of 2^17 of them overflows
+    // the leader's
+    uint32_t list_key[kList], list_index[kList], listed;
+    u64 list_weight[kList];
+    // the leader's answer, to all
+    int bin;
+    uint32_t before_count, in_bin;
+    u64 before_mass;
+    uint32_t key, index;
+    int found, at, abandon;
+};
+
+template <typename T>
+struct Slice {
+    const T* at;              // in shared memory
+    int from, n;              // index of the first, how many
+    float most;               // of the row
+    float depth;              // 2 kBins / (kDepth T): bins per unit of the logits' halves
+    double rate;              // -256 log2(e) / T
+    const double* table;
+    __device__ __forceinline__ float logit(int i) const {
+        const float x = (float)at[i] + 0.f;   // (-0 + 0 = 0: equal logits have equal keys)
+        return x != x ? -INFINITY : x;
+    }
+    // 2^44 e^((x - most) / T), rounded: 2^(k / 256) from the table, the rest by the series of 2^x
+    __device__ __forceinline__ u64 weight(float x) const {
+        if (x == most) return 1ull << 44;
+        if (bin(x) >= kBins - 1) return 0;
+        const double d = (double)most - (double)x, magic = 6755399441055744.0;   // 1.5 x 2^52: a sum's low word is the number, rounded
+        const double t = __fma_rn(d, rate, magic);
+        const int k = -__double2loint(t);   // (>= 0)
+        if (k >= 64 * kTable) return 0;
+        const double r = __fma_rn(d, rate, -(t - magic)) * (1.0 / 256);
+        double p = __fma_rn(r, 0.0096181291076284772, 0.055504108664821580);
+        p = __fma_rn(p, r, 0.24022650695910071);
+        p = __fma_rn(p, r, 0.69314718055994531);
+        p = __fma_rn(p, r, 1.0);
+        const double w = p * table[k & (kTable - 1)];
+        const double scaled = __hiloint2double(__double2hiint(w) - ((k / kTable) << 20), __double2loint(w));
+        return (u64)__double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull;   // + 2^52: a whole number in the low bits
+    }
+    // 0 .. kBins - 1 by falling logit; the last holds what weighs nothing
+    __device__ __forceinline__ int bin(float x) const {
+        if (x == most) return 0;
+        const float b = (0.5f * most - 0.5f * x) * depth;   // (their difference may be too large)
+        return b < (float)(kBins - 1) ? (int)b : kBins - 1;   // (also of -infinity, and under a highest logit of infinity)
+    }
+};
+
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kCta, 2) sample_cluster_kernel(const __grid_constant__ SampleParams p, int slice) {
+    namespace cg = cooperative_groups;
+    extern __shared__ __align__(128) uint8_t raw[];
+    __shared__ ClusterShared sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = cluster.num_blocks(), me = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t r = blockIdx.x / ctas;
+    ClusterShared& leader = *cluster.map_shared_rank(&sh, 0);
+    T* const x = (T*)raw;
+    const int from = me * slice, n = max(0, min(slice, p.vocab - from));
+    const uint32_t bar = tcp::smem_u32(&sh.bar);
+    if (threadIdx.x == 0) {
+        tcp::mbar_init(bar, 1);
+        sh.abandon = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    auto started = cluster.barrier_arrive();   // (a CTA's memory is there once it runs)
+    if (threadIdx.x < kTable) sh.table[threadIdx.x] = exp2(44.0 - (double)threadIdx.x / kTable);
+    __syncthreads();
+    pdl_enter();
+    // ---- the slice
+    const T* in = (const T*)p.logits + r * p.row_stride + from;
+    constexpr int kUnit = 16 / sizeof(T);
+    const bool bulk = p.row_stride % kUnit == 0 && (uintptr_t)p.logits % 16 == 0;   // (slices are multiples of 16 bytes)
+    const int whole = bulk ? n / kUnit * kUnit : 0;
+    if (whole > 0 && threadIdx.x == 0) {
+        tcp::mbar_expect_tx(bar, whole * sizeof(T));
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tcp::smem_u32(x)), "l"(in),
+                     "r"((uint32_t)(whole * sizeof(T))), "r"(bar) : "memory");
+    }
+    for (int i = whole + threadIdx.x; i < n; i += kCta) x[i] = in[i];
+    const float temperature = p.temperature ? p.temperature[r] : 1.f, uniform = p.uniform[r], top_p = p.top_p ? p.top_p[r] : 1.f, min_p = p.min_p ? p.min_p[r] : 0.f;
+    const int top_k = p.top_k ? p.top_k[r] : 0;
+    if (whole > 0) tcp::mbar_wait(bar, 0, &sh.abandon, p.status, 72u);   // (given up: the row is wrong, the host learns of it)
+    __syncthreads();
+    cluster.barrier_wait(std::move(started));
+    // one number from each CTA; all get all of them
+    int turn = 0;
+    const auto exchange = [&](u64 v) {   // by thread 0
+        if (threadIdx.x == 0)
+            for (int c = 0; c < ctas; c++) cluster.map_shared_rank(&sh, c)->slots[turn][me] = v;
+        cluster.sync();
+        return sh.slots[turn++ & 1];
+    };
+    Slice<T> row{x, from, n, 0.f, 0.f, 0.0, sh.table};
+    // ---- highest logit, and where it is first
+    u64 top = 0;
+    for (int i = threadIdx.x; i < n; i += kCta) {
+        const u64 k = (u64)key_of(row.logit(i)) << 32 | (uint32_t)~(from + i);
+        top = top > k ? top : k;
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+        const u64 w = __shfl_xor_sync(0xffffffffu, top, o);
+        top = top > w ? top : w;
+    }
+    if (lane == 0) sh.scan[warp] = top;
+    __syncthreads();
+    for (int w = 0; w < kWarps; w++) top = top > sh.scan[w] ? top : sh.scan[w];
+    {
+        const u64* all = exchange(top);
+        for (int c = 0; c < ctas; c++) top = top > all[c] ? top : all[c];
+        turn &= 1;
+    }
+    const uint32_t top_key = (uint32_t)(top >> 32);
+    const int first = (int)~(uint32_t)top;
+    row.most = __uint_as_float(top_key & 0x80000000u ? top_key & 0x7fffffffu : ~top_key);
+    if (row.most == -INFINITY || !(temperature > 0.f)) {
+        if (me == 0 && threadIdx.x == 0) p.out[r] = row.most == -INFINITY ? -1 : first;
+        return;   // (all CTAs of the cluster; nobody reads another's memory any more)
+    }
+    row.rate = -256.0 * 1.4426950408889634074 / (double)temperature;
+    row.depth = fminf(2.f * (float)kBins / kDepth / temperature, 1e30f);
+    Cut cut{0, INT_MAX};
+
+    // In the order of the index: what each piece weighs by `amount`, summed over the cluster; then the first index at which the
+    // running sum passes `goal` (a sum reaches it where `reach`).  Its number goes to all CTAs
+    const int piece = (slice + kWarps * kPieces - 1) / (kWarps * kPieces);
+    const auto sums = [&](auto amount) {
+        for (int q = 0; q < kPieces; q++) {
+            const int a = (warp * kPieces + q) * piece, b = min(n, a + piece);
+            u64 sum = 0;
+            for (int i = a + lane; i < b; i += 32) sum += amount(row.logit(i), from + i);
+            sum = warp_sum(sum);
+            if (lane == 0) sh.pieces[warp * kPieces + q] = sum;
+        }
+        __syncthreads();
+        u64 all = threadIdx.x < kWarps * kPieces ? sh.pieces[threadIdx.x] : 0;
+        all = warp_sum(all);
+        if (lane == 0) sh.scan[warp] = all;
+        __syncthreads();
+        all = 0;
+        for (int w = 0; w < kWarps * kPieces / 32; w++) all += sh.scan[w];
+        return all;   // of this CTA
+    };
+    const auto search = [&](auto amount, auto passes, u64 front, u64 own) {   // front: of the CTAs in front, own: this one's
+        if (own == 0 || !passes(front + own) || (front > 0 && passes(front))) return -1;   // (only the CTA in which it happens)
+        if (threadIdx.x == 0) {
+            u64 run = front;
+            int q = 0;
+            for (; q < kWarps * kPieces - 1; q++) {
+                if (passes(run + sh.pieces[q])) break;
+                run += sh.pieces[q];
+            }
+            sh.before_mass = run;
+            sh.found = q;
+            sh.at = -1;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            u64 run = sh.before_mass;
+            const int a = sh.found * piece, b = min(n, a + piece);
+            for (int i0 = a; i0 < b; i0 += 32) {
+                const int i = i0 + lane;
+                const u64 v = i < b ? amount(row.logit(i), from + i) : 0;
+                u64 up = v;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 w = __shfl_up_sync(0xffffffffu, up, o);
+                    if (lane >= o) up += w;
+                }
+                const uint32_t over = __ballot_sync(0xffffffffu, v > 0 && passes(run + up));
+                if (over) {
+                    if (lane == 0) sh.at = from + i0 + __ffs(over) - 1;
+                    break;
+                }
+                run += __shfl_sync(0xffffffffu, up, 31);
+            }
+        }
+        __syncthreads();
+        return sh.at;
+    };
+
+    // ---- a cut: the shortest head of the order, within `within`, of `k` tokens or of `share` of the weight (k == 0)
+    const auto find_cut = [&](Cut within, int k, double share) {
+        // bins: first of the logits, then, while one holds more tokens than the list, of their keys from low to high
+        uint32_t low = 0, high = 0xffffffffu, before_count = 0;
+        u64 before_mass = 0, goal = 0;
+        int bin = -1;
+        for (int level = 0;; level++) {
+            const uint64_t range = (uint64_t)high - low + 1;
+            const auto bin_of = [&](float x, uint32_t key) { return level == 0 ? row.bin(x) : (int)((uint64_t)(high - key) * kBins / range); };
+            const auto member = [&](float x, uint32_t key, int i) { return within.keeps(key, i) && (level == 0 || (row.bin(x) == bin && key >= low && key <= high)); };
+            for (int i = threadIdx.x; i < kBins; i += kCta) sh.counts[i] = sh.limbs[0][i] = sh.limbs[1][i] = sh.limbs[2][i] = 0;
+            if (threadIdx.x == 0) sh.listed = 0;
+            __syncthreads();
+            for (int i = threadIdx.x; i < n; i += kCta) {
+                const float v = row.logit(i);
+                const uint32_t key = key_of(v);
+                if (!member(v, key, from + i)) continue;
+                const int b = bin_of(v, key);
+                if (level == 0 && b == kBins - 1) continue;   // weighs nothing
+                atomicAdd(&sh.counts[b], 1u);
+                if (k == 0) {
+                    const u64 w = row.weight(v);
+                    atomicAdd(&sh.limbs[0][b], (uint32_t)w & 0x7fffu);
+                    atomicAdd(&sh.limbs[1][b], (uint32_t)(w >> 15) & 0x7fffu);
+                    atomicAdd(&sh.limbs[2][b], (uint32_t)(w >> 30));
+                }
+            }
+            cluster.sync();
+            if (me == 0) {
+                // two bins a thread: their sums, those of all in front, and where the goal is reached
+                Amount mine[2];
+                for (int j = 0; j < 2; j++) {
+                    const int b = 2 * threadIdx.x + j;
+                    mine[j] = {0, 0};
+                    for (int c = 0; c < ctas; c++) {
+                        const ClusterShared& o = *cluster.map_shared_rank(&sh, c);
+                        mine[j].count += o.counts[b];
+                        mine[j].mass += (u64)o.limbs[0][b] + ((u64)o.limbs[1][b] << 15) + ((u64)o.limbs[2][b] << 30);
+                    }
+                }
+                const u64 measure[2] = {k > 0 ? mine[0].count : mine[0].mass, k > 0 ? mine[1].count : mine[1].mass};
+                u64 up = measure[0] + measure[1];
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 w = __shfl_up_sync(0xffffffffu, up, o);
+                    if (lane >= o) up += w;
+                }
+                __syncthreads();
+                if (lane == 31) sh.scan[warp] = up;
+                if (threadIdx.x == 0) sh.bin = -1;
+                __syncthreads();
+                u64 all = 0;
+                for (int w = 0; w < kWarps; w++) {
+                    if (w < warp) up += sh.scan[w];
+                    all += sh.scan[w];
+                }
+                if (level == 0) {
+                    const double g = ceil(share * (double)all);
+                    goal = k > 0 ? (u64)k : g >= 1.0 ? (u64)g : 1;
+                }
+                u64 run = (k > 0 ? before_count : before_mass) + up - measure[0] - measure[1];
+                for (int j = 0; j < 2; j++) {
+                    if (measure[j] > 0 && run < goal && goal <= run + measure[j]) {
+                        sh.bin = 2 * threadIdx.x + j;
+                        sh.before_mass = run;
+                        sh.in_bin = mine[j].count;
+                    }
+                    run += measure[j];
+                }
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    const u64 run0 = sh.before_mass, g = goal;
+                    const int b = sh.bin;
+                    const uint32_t in_bin = sh.in_bin;
+                    for (int c = 0; c < ctas; c++) {
+                        ClusterShared& o = *cluster.map_shared_rank(&sh, c);
+                        o.bin = b, o.before_mass = run0, o.in_bin = in_bin, o.scan[0] = g;
+                    }
+                }
+            }
+            cluster.sync();
+            if (sh.bin < 0) return within;   // all that weighs anything stays
+            goal = sh.scan[0];
+            if (k > 0) before_count = (uint32_t)sh.before_mass;
+            else before_mass = sh.before_mass;
+            const int chosen = sh.bin;
+            const uint32_t in_bin = sh.in_bin;
+            const uint32_t old_high = high;
+            if (level == 0) {
+                bin = chosen;
+            } else {
+                // keys of which (high - key) kBins / range is `chosen`
+                const uint64_t near = ((uint64_t)chosen * range + kBins - 1) / kBins, far = ((uint64_t)(chosen + 1) * range + kBins - 1) / kBins - 1;
+                high = old_high - (uint32_t)near;
+                low = old_high - (uint32_t)far;
+            }
+            const auto chosen_one = [&](float v, uint32_t key, int i) { return within.keeps(key, i) && row.bin(v) == bin && key >= low && key <= high; };
+            if (in_bin <= kList) {
+                // to the leader, who finds each one's place among them
+                for (int i = threadIdx.x; i < n; i += kCta) {
+                    const float v = row.logit(i);
+                    const uint32_t key = key_of(v);
+                    if (!chosen_one(v, key, from + i)) continue;
+                    const uint32_t at = atomicAdd(&leader.listed, 1u);
+                    leader.list_key[at] = key, leader.list_index[at] = from + i, leader.list_weight[at] = k > 0 ? 1 : row.weight(v);
+                }
+                cluster.sync();
+                if (me == 0)
+                    for (uint32_t e = threadIdx.x; e < in_bin; e += kCta) {
+                        const uint32_t key = sh.list_key[e], index = sh.list_index[e];
+                        u64 run = k > 0 ? before_count : before_mass;
+                        for (uint32_t o = 0; o < in_bin; o++) {
+                            const uint32_t other = sh.list_key[o];
+                            if (other > key || (other == key && sh.list_index[o] < index)) run += sh.list_weight[o];
+                        }
+                        if (run < goal && goal <= run + sh.list_weight[e])
+                            for (int c = 0; c < ctas; c++) {
+                                ClusterShared& o = *cluster.map_shared_rank(&sh, c);
+                                o.key = key, o.index = index;
+                            }
+                    }
+                cluster.sync();
+                const Cut found{sh.key, (int)sh.index};
+                cluster.sync();   // (before anybody writes there again)
+                return found;
+            }
+            if (low == high) {
+                // equal logits: by index
+                float value = 0.f;
+                const uint32_t key = low;
+                value = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+                const u64 each = k > 0 ? 1 : row.weight(value), need = (goal - (k > 0 ? before_count : before_mass) + each - 1) / each;
+                const auto one = [&](float v, int i) { return (u64)(key_of(v) == key && within.keeps(key, i) ? 1 : 0); };
+                const u64 own = sums(one);
+                const u64* all = exchange(own);
+                turn &= 1;
+                u64 front = 0;
+                for (int c = 0; c < me; c++) front += all[c];
+                const int at = search(one, [&](u64 s) { return s >= need; }, front, own);
+                if (at >= 0 && threadIdx.x == 0)
+                    for (int c = 0; c < ctas; c++) cluster.map_shared_rank(&sh, c)->index = at;
+                cluster.sync();
+                const Cut found{key, (int)sh.index};
+                cluster.sync();
+                return found;
+            }
+            if (level == 0) {
+                // the keys of that bin
+                uint32_t lo = 0xffffffffu, hi = 0;
+                for (int i = threadIdx.x; i < n; i += kCta) {
+                    const float v = row.logit(i);
+                    const uint32_t key = key_of(v);
+                    if (!chosen_one(v, key, from + i)) continue;
+                    lo = min(lo, key), hi = max(hi, key);
+                }
+                lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
+                __syncthreads();
+                if (lane == 0) sh.scan[warp] = (u64)lo << 32 | hi;
+                __syncthreads();
+                for (int w = 0; w < kWarps; w++) lo = min(lo, (uint32_t)(sh.scan[w] >> 32)), hi = max(hi, (uint32_t)sh.scan[w]);
+                const u64* all = exchange((u64)lo << 32 | hi);
+                turn &= 1;
+                for (int c = 0; c < ctas; c++) lo = min(lo, (uint32_t)(all[c] >> 32)), hi = max(hi, (uint32_t)all[c]);
+                low = lo, high = hi;
+            }
+        }
+    };
+    if (top_k > 0 && top_k < p.vocab) cut = find_cut(cut, top_k, 0.0);
+    if (p.top_p && !(top_p >= 1.f)) cut = find_cut(cut, 0, (double)top_p);
+
+    // ---- the token
+    const double least_weight = (double)min_p * 17592186044416.0;
+    const auto amount = [&](float v, int i) {
+        if (i != first && !cut.keeps(key_of(v), i)) return (u64)0;
+        const u64 w = row.weight(v);
+        return i == first || (double)w >= least_weight ? w : (u64)0;
+    };
+    const u64 own = sums(amount);
+    const u64* all = exchange(own);
+    u64 front = 0, total = 0;
+    for (int c = 0; c < ctas; c++) {
+        if (c < me) front += all[c];
+        total += all[c];
+    }
+    const double goal = fmax((double)uniform * (double)total, 0.0);
+    const auto passes = [&](u64 s) { return (double)s > goal || s == total; };   // (the last token for a number of 1 and more)
+    const int token = search(amount, passes, front, own);
+    if (token >= 0 && threadIdx.x == 0) p.out[r] = token;
+    cluster.sync();   // (nobody leaves while another may still read its memory)
+}
+
+// CTAs of a row's cluster and tokens of each; 0: the row does not fit
+int cluster_of(const SampleParams& p, int* slice) {
+    const int size = p.half ? 2 : 4, unit = 16 / size;
+    const auto tokens = [&](int ctas) { return ((p.vocab + ctas - 1) / ctas + unit - 1) / unit * unit; };
+    int ctas = 1;
+    // 64 KB a CTA, for two on an SM; and, of few rows, as many CTAs as have an SM's half, with 1024 tokens and more each
+    while (ctas < kMaxCluster && ((int64_t)tokens(ctas) * size > 64 * 1024 || (p.rows * ctas * 2 <= 2 * 148 && p.vocab / (2 * ctas) >= 1024))) ctas *= 2;
+    *slice = tokens(ctas);
+    return p.col_stride != 1 || (int64_t)*slice * size > 180 * 1024 || p.rows * ctas > INT_MAX ? 0 : ctas;
+}
+
+template <typename T>
+int launch_cluster(const SampleParams& p, int ctas, int slice, cudaStream_t stream) {
+    static bool done[64];
+    static std::mutex mu;
+    const int err = allow_shared(sample_cluster_kernel<T>, 180 * 1024, done, mu);
+    if (err != 0) return err;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.rows * ctas));
+    cfg.blockDim = dim3(kCta);
+    cfg.dynamicSmemBytes = (size_t)slice * sizeof(T);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    (void)cudaLaunchKernelEx(&cfg, sample_cluster_kernel<T>, p, slice);   // a failure stays in cudaGetLastError()
+    return 0;
+}
+
 }  // namespace
 
 int launch_sample(const SampleParams& p, cudaStream_t stream) {
+    int slice = 0;
+    if (const int ctas = cluster_of(p, &slice)) {
+        const int err = p.half ? launch_cluster<__half>(p, ctas, slice, stream) : launch_cluster<float>(p, ctas, slice, stream);
+        return err != 0 ? err : (int)cudaGetLastError();
+    }
     const dim3 grid((unsigned)std::min<int64_t>(p.rows, 1 << 20));
     if (p.half) launch_pdl(sample_kernel<__half>, grid, dim3(kThreads), 0, stream, p);
     else launch_pdl(sample_kernel<float>, grid, dim3(kThreads), 0, stream, p);

@@ -552,6 +552,30 @@ def test_sample_among_equals():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("spread", [1e-6, 1e-3, 0.05])
+def test_sample_of_logits_close_together(dtype, spread):
+    """Thousands of tokens between which a cut falls, of few different logits or of many"""
+    rng = np.random.default_rng(7)
+    rows, vocab = 12, 20011
+    logits = (5 + spread * rng.standard_normal((rows, vocab))).astype(dtype.np)
+    uniform = rng.random(rows, dtype=np.float32)
+    for given in (dict(top_k=rng.integers(1, vocab, rows).astype(np.int32)), dict(top_p=rng.uniform(0.05, 0.95, rows).astype(np.float32)),
+                  dict(top_k=rng.integers(2000, vocab, rows).astype(np.int32), top_p=rng.uniform(0.05, 0.95, rows).astype(np.float32), min_p=np.full(rows, 0.9, np.float32))):
+        assert np.array_equal(sample(logits, uniform, **given), plain_sample(logits, uniform, **given)), given
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, rows, vocab", [(F32, 2, 1 << 19), (F16, 2, 1 << 19), (F32, 1, 8 * 46080 + 1), (F16, 333, 2048), (F32, 700, 5)])
+def test_sample_of_the_largest_vocabularies_and_many_rows(dtype, rows, vocab):
+    rng = np.random.default_rng(vocab)
+    logits = (4 * rng.standard_normal((rows, vocab))).astype(dtype.np)
+    uniform = rng.random(rows, dtype=np.float32)
+    given = dict(temperature=rng.uniform(0.5, 2, rows).astype(np.float32), top_p=rng.uniform(0.3, 1.1, rows).astype(np.float32))
+    assert np.array_equal(sample(logits, uniform, **given), plain_sample(logits, uniform, **given))
+
+
+@pytest.mark.gpu
 def test_sample_without_weights():
     """Rows of nothing but -infinity or NaN; infinities share all of the weight; temperatures from far below to far above 1"""
     vocab = 777
