@@ -14,7 +14,9 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
+#include <type_traits>
 
 #include "../kernels.h"
 #include "launch.cuh"
@@ -250,6 +252,7 @@ struct Slice {
     const T* at;              // in shared memory
     int from, n;              // index of the first, how many
     float most;               // of the row
+    float least;              // logits below it weigh nothing
     float depth;              // 2 kBins / (kDepth T): bins per unit of the logits' halves
     double rate;              // -256 log2(e) / T
     const double* table;
@@ -257,22 +260,25 @@ struct Slice {
         const float x = (float)at[i] + 0.f;   // (-0 + 0 = 0: equal logits have equal keys)
         return x != x ? -INFINITY : x;
     }
-    // 2^44 e^((x - most) / T), rounded: 2^(k / 256) from the table, the rest by the series of 2^x
-    __device__ __forceinline__ u64 weight(float x) const {
-        if (x == most) return 1ull << 44;
-        if (bin(x) >= kBins - 1) return 0;
-        const double d = (double)most - (double)x, magic = 6755399441055744.0;   // 1.5 x 2^52: a sum's low word is the number, rounded
+    // 2^44 e^((x - most) / T), rounded, + 2^52, as the bits of an f64: the number is in the low 52.  2^(k / 256) from the table, the rest
+    // by the series of 2^x.  (Finite `most`; of NaN, and of -infinity where `least` is above the lowest number, 0)
+    __device__ __forceinline__ u64 weight_bits(float x) const {
+        const double d = (double)most - (double)fmaxf(x, least), magic = 6755399441055744.0;   // 1.5 x 2^52: a sum's low word is the number, rounded
         const double t = __fma_rn(d, rate, magic);
-        const int k = -__double2loint(t);   // (>= 0)
-        if (k >= 64 * kTable) return 0;
-        const double r = __fma_rn(d, rate, -(t - magic)) * (1.0 / 256);
-        double p = __fma_rn(r, 0.0096181291076284772, 0.055504108664821580);
-        p = __fma_rn(p, r, 0.24022650695910071);
-        p = __fma_rn(p, r, 0.69314718055994531);
+        const int k = -__double2loint(t);   // (0 to 64 x 256)
+        const double r = __fma_rn(d, rate, -(t - magic));   // 256 times the rest, up to 1/2 either way
+        constexpr double kLn = 0.69314718055994531 / 256;
+        double p = __fma_rn(r, kLn * kLn * kLn * kLn / 24, kLn * kLn * kLn / 6);
+        p = __fma_rn(p, r, kLn * kLn / 2);
+        p = __fma_rn(p, r, kLn);
         p = __fma_rn(p, r, 1.0);
         const double w = p * table[k & (kTable - 1)];
-        const double scaled = __hiloint2double(__double2hiint(w) - ((k / kTable) << 20), __double2loint(w));
-        return (u64)__double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull;   // + 2^52: a whole number in the low bits
+        const double scaled = __hiloint2double(__double2hiint(w) - (int)((uint32_t)(k << 12) & 0xfff00000u), __double2loint(w));
+        return (u64)__double_as_longlong(scaled + 4503599627370496.0);
+    }
+    __device__ __forceinline__ u64 weight(float x) const {
+        if (most == INFINITY) return x == most ? 1ull << 44 : 0;
+        return x > -INFINITY ? weight_bits(x) & 0xfffffffffffffull : 0;
     }
     // 0 .. kBins - 1 by falling logit; the last holds what weighs nothing
     __device__ __forceinline__ int bin(float x) const {
@@ -319,6 +325,7 @@ __global__ void __launch_bounds__(kCta, 2) sample_cluster_kernel(const __grid_co
                      "r"((uint32_t)(whole * sizeof(T))), "r"(bar) : "memory");
     }
     for (int i = whole + threadIdx.x; i < n; i += kCta) x[i] = in[i];
+    if (threadIdx.x == 0 && (n & 1)) x[n] = (T)-INFINITY;
     const float temperature = p.temperature ? p.temperature[r] : 1.f, uniform = p.uniform[r], top_p = p.top_p ? p.top_p[r] : 1.f, min_p = p.min_p ? p.min_p[r] : 0.f;
     const int top_k = p.top_k ? p.top_k[r] : 0;
     if (whole > 0) tcp::mbar_wait(bar, 0, &sh.abandon, p.status, 72u);   // (given up: the row is wrong, the host learns of it)
@@ -332,44 +339,66 @@ __global__ void __launch_bounds__(kCta, 2) sample_cluster_kernel(const __grid_co
         cluster.sync();
         return sh.slots[turn++ & 1];
     };
-    Slice<T> row{x, from, n, 0.f, 0.f, 0.0, sh.table};
-    // ---- highest logit, and where it is first
-    u64 top = 0;
-    for (int i = threadIdx.x; i < n; i += kCta) {
-        const u64 k = (u64)key_of(row.logit(i)) << 32 | (uint32_t)~(from + i);
-        top = top > k ? top : k;
+    Slice<T> row{x, from, n, 0.f, 0.f, 0.f, 0.0, sh.table};
+    // ---- highest logit
+    using Two = typename std::conditional<sizeof(T) == 2, __half2, float2>::type;
+    const auto two_of = [&](int i) {   // logits 2 i and 2 i + 1 of the slice
+        const Two v = ((const Two*)x)[i];
+        if constexpr (sizeof(T) == 2) return __half22float2(v);
+        else return v;
+    };
+    const int pairs = (n + 1) / 2;   // (what is behind the last is -infinity)
+    float most = -INFINITY;
+    for (int i = threadIdx.x; i < pairs; i += kCta) {
+        const float2 v = two_of(i);
+        most = fmaxf(most, fmaxf(v.x, v.y));
     }
-    for (int o = 16; o > 0; o >>= 1) {
-        const u64 w = __shfl_xor_sync(0xffffffffu, top, o);
-        top = top > w ? top : w;
-    }
-    if (lane == 0) sh.scan[warp] = top;
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) sh.scan[warp] = __float_as_uint(most);
     __syncthreads();
-    for (int w = 0; w < kWarps; w++) top = top > sh.scan[w] ? top : sh.scan[w];
+    for (int w = 0; w < kWarps; w++) most = fmaxf(most, __uint_as_float((uint32_t)sh.scan[w]));
     {
-        const u64* all = exchange(top);
-        for (int c = 0; c < ctas; c++) top = top > all[c] ? top : all[c];
+        const u64* all = exchange(__float_as_uint(most));
+        for (int c = 0; c < ctas; c++) most = fmaxf(most, __uint_as_float((uint32_t)all[c]));
         turn &= 1;
     }
-    const uint32_t top_key = (uint32_t)(top >> 32);
-    const int first = (int)~(uint32_t)top;
-    row.most = __uint_as_float(top_key & 0x80000000u ? top_key & 0x7fffffffu : ~top_key);
-    if (row.most == -INFINITY || !(temperature > 0.f)) {
-        if (me == 0 && threadIdx.x == 0) p.out[r] = row.most == -INFINITY ? -1 : first;
+    row.most = most + 0.f;
+    if (most == -INFINITY) {
+        if (me == 0 && threadIdx.x == 0) p.out[r] = -1;
         return;   // (all CTAs of the cluster; nobody reads another's memory any more)
     }
+    if (!(temperature > 0.f) || min_p > 1.f) {
+        // the first of the highest is all that stays
+        uint32_t first = 0xffffffffu;
+        for (int i = threadIdx.x; i < n; i += kCta)
+            if (row.logit(i) == row.most) first = min(first, (uint32_t)(from + i));
+        first = __reduce_min_sync(0xffffffffu, first);
+        __syncthreads();
+        if (lane == 0) sh.scan[warp] = first;
+        __syncthreads();
+        for (int w = 0; w < kWarps; w++) first = min(first, (uint32_t)sh.scan[w]);
+        const u64* all = exchange(first);
+        for (int c = 0; c < ctas; c++) first = min(first, (uint32_t)all[c]);
+        if (me == 0 && threadIdx.x == 0) p.out[r] = (int)first;
+        return;
+    }
     row.rate = -256.0 * 1.4426950408889634074 / (double)temperature;
+    row.least = fmaxf(row.most - 44.f * temperature, -FLT_MAX);   // (e^-44 is 2^-63)
     row.depth = fminf(2.f * (float)kBins / kDepth / temperature, 1e30f);
     Cut cut{0, INT_MAX};
 
     // In the order of the index: what each piece weighs by `amount`, summed over the cluster; then the first index at which the
     // running sum passes `goal` (a sum reaches it where `reach`).  Its number goes to all CTAs
-    const int piece = (slice + kWarps * kPieces - 1) / (kWarps * kPieces);
-    const auto sums = [&](auto amount) {
+    const int piece = (slice + 2 * kWarps * kPieces - 1) / (2 * kWarps * kPieces) * 2;
+    const auto sums = [&](auto amount, u64 bias = 0) {   // bias: what each amount is too large by
         for (int q = 0; q < kPieces; q++) {
             const int a = (warp * kPieces + q) * piece, b = min(n, a + piece);
             u64 sum = 0;
-            for (int i = a + lane; i < b; i += 32) sum += amount(row.logit(i), from + i);
+            for (int i = a / 2 + lane; 2 * i < b; i += 32) {
+                const float2 v = two_of(i);
+                sum += amount(v.x, from + 2 * i) + amount(v.y, from + 2 * i + 1);
+            }
+            if (b > a) sum -= bias * (2 * (u64)max(0, (((b + 1) / 2 - a / 2) - lane + 31) / 32));
             sum = warp_sum(sum);
             if (lane == 0) sh.pieces[warp * kPieces + q] = sum;
         }
@@ -550,7 +579,7 @@ __global__ void __launch_bounds__(kCta, 2) sample_cluster_kernel(const __grid_co
                 const uint32_t key = low;
                 value = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
                 const u64 each = k > 0 ? 1 : row.weight(value), need = (goal - (k > 0 ? before_count : before_mass) + each - 1) / each;
-                const auto one = [&](float v, int i) { return (u64)(key_of(v) == key && within.keeps(key, i) ? 1 : 0); };
+                const auto one = [&](float v, int i) { return (u64)(key_of(v + 0.f) == key && within.keeps(key, i) ? 1 : 0); };
                 const u64 own = sums(one);
                 const u64* all = exchange(own);
                 turn &= 1;
@@ -589,13 +618,15 @@ __global__ void __launch_bounds__(kCta, 2) sample_cluster_kernel(const __grid_co
     if (p.top_p && !(top_p >= 1.f)) cut = find_cut(cut, 0, (double)top_p);
 
     // ---- the token
-    const double least_weight = (double)min_p * 17592186044416.0;
+    const u64 least_weight = (u64)ceil(fmax((double)min_p, 0.0) * 17592186044416.0);
+    const bool all_stay = cut.key == 0;
     const auto amount = [&](float v, int i) {
-        if (i != first && !cut.keeps(key_of(v), i)) return (u64)0;
         const u64 w = row.weight(v);
-        return i == first || (double)w >= least_weight ? w : (u64)0;
+        return w >= least_weight && (all_stay || cut.keeps(key_of(v + 0.f), i)) ? w : (u64)0;
     };
-    const u64 own = sums(amount);
+    // (all tokens, the usual kind: no more than their weights)
+    const bool usual = all_stay && least_weight == 0 && row.most < INFINITY && row.least > -FLT_MAX;
+    const u64 own = usual ? sums([&](float v, int) { return row.weight_bits(v); }, 0x4330000000000000ull) : sums(amount);
     const u64* all = exchange(own);
     u64 front = 0, total = 0;
     for (int c = 0; c < ctas; c++) {
