@@ -272,26 +272,27 @@ class LlamaBlocks:
     tensor-parallel builder (kyanite_b200/tensor_parallel.py), which uses them on weight slices."""
 
     def __init__(self, g: Graph, d_model: int, head_dim: int, seq: int, eps: float, rope_base: float,
-                 dtype: DType = DType.F32):
-        """`dtype`: the storage type of activations and weights, F32 or F16.  With F16 every value of the graph is
+                 dtype: DType = DType.F32, tables: bool = True):
+        """`tables`: positions are 0 to seq - 1, under a causal mask; else the caller sets `cos` and `sin`.  `dtype`: the storage type of activations and weights, F32 or F16.  With F16 every value of the graph is
         f16 except inside RMSNorm, whose statistics are computed on f32 casts (as half-precision decoders do) and
         whose result is cast back."""
         self.g, self.d_model, self.hd, self.seq, self.eps, self.dtype = g, d_model, head_dim, seq, eps, dtype
-        cos, sin = rope_tables(seq, head_dim, rope_base)
-        self.cos, self.sin = g.constant_tensor(cos.astype(dtype.np)), g.constant_tensor(sin.astype(dtype.np))
-        self.mask = g.constant_tensor(np.triu(np.full((seq, seq), -np.inf, dtype.np), 1).reshape(1, seq, seq))
+        if tables:
+            cos, sin = rope_tables(seq, head_dim, rope_base)
+            self.cos, self.sin = g.constant_tensor(cos.astype(dtype.np)), g.constant_tensor(sin.astype(dtype.np))
+            self.mask = g.constant_tensor(np.triu(np.full((seq, seq), -np.inf, dtype.np), 1).reshape(1, seq, seq))
         self.rows = BATCH * seq
 
     def linear(self, x: Value, w: np.ndarray) -> Value:
         return self.g.linear(x, self.g.constant_tensor(np.ascontiguousarray(w, dtype=self.dtype.np)))
 
-    def rmsnorm(self, t: Value, gain: np.ndarray) -> Value:
-        """t [B, seq, d_model]: composed from pow / mean / sqrt / div (the IR has no RMSNorm)."""
+    def rmsnorm(self, t: Value, gain: np.ndarray, seq: int = None) -> Value:
+        """t [B, seq, d_model] (`seq`: the graph's unless given): composed from pow / mean / sqrt / div (the IR has no RMSNorm)."""
         from .graph import BinaryOp, ReduceOp, UnaryOp
         g = self.g
         if self.dtype != DType.F32:
             t = g.value_cast(t, DType.F32)
-        ms = g.view(g.reduce(g.pow(t, g.scalar(2.0)), [2], ReduceOp.MEAN), shape(BATCH, self.seq, 1))
+        ms = g.view(g.reduce(g.pow(t, g.scalar(2.0)), [2], ReduceOp.MEAN), shape(BATCH, seq or self.seq, 1))
         rms = g.unary(UnaryOp.SQRT, g.add(ms, g.scalar(self.eps)))
         out = g.mul(g.binary(BinaryOp.DIV, t, rms), g.constant_tensor(gain))
         return out if self.dtype == DType.F32 else g.value_cast(out, self.dtype)
@@ -367,6 +368,48 @@ def llama_decoder(layers: int = 32, d_model: int = 4096, heads: int = 32, ffn: i
         return [_rng(seed).integers(0, vocab, (batch_size, seq)).astype(np.int32)]
 
     return g, make_inputs
+
+
+def llama_answer(tokens: int, capacity: int, layers: int = 32, d_model: int = 4096, heads: int = 32, ffn: int = 11008, vocab: int = 32000,
+                 eps: float = 1e-6, rope_base: float = 10000.0, seed: int = 10, dtype: DType = DType.F16, cache_dtype: DType = DType.I8,
+                 with_logits: bool = False) -> Graph:
+    """The LLaMA-shaped decoder as it answers: `tokens` new tokens of every sequence go behind what the caches hold of it (one cache per
+    layer, `capacity` positions, attached with `CudaExecutor.set_cache`), and one token is drawn for each sequence.  The weights
+    are `llama_decoder`'s.  Inputs: token ids [B, tokens] (i32); positions before them [B] (i32); how many of them count [B]
+    (i32); the row of each sequence's last one among all B * tokens (i32 [B]: `answer_rows`); random numbers, temperature, top-k
+    (i32) and top-p [B] (`Graph.sample`).  Outputs: tokens [B] (i32) and, `with_logits`, the logits they were drawn from [B, vocab]."""
+    g = Graph()
+    w = llama_weights(layers, d_model, heads, ffn, vocab, seed)
+    hd = d_model // heads
+    blocks = LlamaBlocks(g, d_model, hd, tokens, eps, rope_base, dtype, tables=False)
+    ids, start, count, last = g.input(shape(BATCH, tokens), DType.I32), g.input(shape(BATCH), DType.I32), g.input(shape(BATCH), DType.I32), g.input(shape(BATCH), DType.I32)
+    uniform, temperature = g.input(shape(BATCH)), g.input(shape(BATCH))
+    top_k, top_p = g.input(shape(BATCH), DType.I32), g.input(shape(BATCH))
+    positions = g.flatten(g.add(g.view(start, shape(BATCH, 1)), g.constant_tensor(np.arange(tokens, dtype=np.int32).reshape(1, tokens))), 0)
+    blocks.cos, blocks.sin = (g.view(g.gather(g.constant_tensor(t.reshape(capacity, hd).astype(dtype.np)), 0, positions), shape(BATCH, tokens, 1, hd))
+                              for t in rope_tables(capacity, hd, rope_base))
+    x = g.view(g.gather(g.constant_tensor(w["table"].astype(dtype.np)), 0, g.flatten(ids, 0)), shape(BATCH, tokens, d_model))
+    heads_shape = shape(BATCH, tokens, heads, hd)
+    for layer in w["layers"]:
+        h = g.view(blocks.rmsnorm(x, layer["norm1"]), shape(blocks.rows, d_model))
+        q, k = (g.view(blocks.rope(blocks.linear(h, layer[name]), heads), heads_shape) for name in ("wq", "wk"))
+        v = g.view(blocks.linear(h, layer["wv"]), heads_shape)
+        cache = g.cache_write(g.cache(BATCH, heads, capacity, hd, cache_dtype), k, v, start, count)
+        ctx = g.view(g.cache_attention(q, cache, start, count), shape(blocks.rows, d_model))
+        x = g.add(x, g.view(blocks.linear(ctx, layer["wo"]), shape(BATCH, tokens, d_model)))
+        x = g.add(x, blocks.ffn_partial(x, layer, slice(0, ffn)))
+    x = g.gather(g.view(x, shape(blocks.rows, d_model)), 0, last)
+    logits = g.linear(g.view(blocks.rmsnorm(g.view(x, shape(BATCH, 1, d_model)), w["norm_f"], 1), shape(BATCH, d_model)),
+                      g.constant_tensor(np.ascontiguousarray(w["lm_head"], dtype=dtype.np)))
+    g.output(g.sample(logits, uniform, temperature, top_k, top_p))
+    if with_logits:
+        g.output(logits)
+    return g
+
+
+def answer_rows(count: np.ndarray, tokens: int) -> np.ndarray:
+    """The rows of the sequences' last tokens for `llama_answer`."""
+    return (np.arange(len(count)) * tokens + np.maximum(count, 1) - 1).astype(np.int32)
 
 
 # --------------------------------------------------------------------------------------
