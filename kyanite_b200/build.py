@@ -46,6 +46,7 @@ SOURCES = [
     "kernels/flash.cu",
     "kernels/cache.cu",
     "kernels/cache_attention.cu",
+    "kernels/cache_attention_rows.cu",
     "kernels/sample.cu",
 ]
 

@@ -316,10 +316,11 @@ struct Executor {
                         p.prefix = cache_at(p.prefix, s.operands[at++]);
                         p.prefix_length = (const int32_t*)ptr[at++];
                     }
-                    if (at < ptr.size()) {
+                    if (s.optional.partial) {
                         p.partial = (float*)ptr[at++];
                         p.arrived = (uint32_t*)ptr[at++];
                     }
+                    if (at < ptr.size()) p.pre = (float*)ptr[at++];
                     p.status = status_dev;
                     const int unit = p.half ? 8 : 4;   // elements of 16 bytes
                     p.q_wide = p.q_strides[3] == 1 && p.cache.dim % unit == 0 && (uintptr_t)p.query % 16 == 0;

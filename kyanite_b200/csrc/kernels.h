@@ -329,11 +329,22 @@ struct CacheAttentionParams {
     int32_t window, tokens, heads, half;
     int32_t q_wide;                // queries' channels can be read 16 bytes at a time
     int32_t grid;                  // CTAs (cache_attention_plan)
+    // rows of 128 at a time (kernels/cache_attention_rows.cu): 0 not, 1 all of it, 2 the prefix, whose parts cache_attention_kernel joins
+    int32_t many, splits, row_items;
+    float* pre;                    // parts: per item and split 256 rows of the channels, reference and sum
 };
+struct CacheRowsPlan {
+    int32_t splits;
+    int64_t items, part_floats;
+};
+CacheRowsPlan cache_attention_rows_plan(const CacheAttentionParams& p, int many);
+int launch_cache_attention_rows(const CacheAttentionParams& p, cudaStream_t stream);
+constexpr int kManyRows = 64, kManyKeys = 256;   // from which on rows are taken 128 at a time
 struct CacheAttentionPlan {
     int32_t grid;
     int64_t items, partial_floats;
     double units;                  // of work, where every sequence is as long as the cache: below 2^31
+    int64_t part_floats;           // of CacheRowsPlan
 };
 CacheAttentionPlan cache_attention_plan(const CacheAttentionParams& p);
 

@@ -108,7 +108,7 @@ __device__ __forceinline__ Span span_of(const CacheAttentionParams& p, int s, in
     const int64_t pre_first = max(seen, (int64_t)0);
     z.pre_tile = z.own_tile = z.pre_tiles = z.tiles = 0;
     if (z.t_lo >= z.t_hi) return z;
-    if (pre_first < shared) {
+    if (pre_first < shared && p.many != 2) {   // (else others see to the prefix)
         z.pre_tile = (int)(pre_first / kTile);
         z.pre_tiles = (shared + kTile - 1) / kTile - z.pre_tile;
     }
@@ -710,9 +710,28 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
         const int64_t slot = 2 * (int64_t)blockIdx.x + (most > 0 || u == u0 ? 0 : 1);
         float* const partial = p.partial + slot * (G::kRows * (kDim + 2));
         const int rows_here = min(G::kRows, rows - row0);
-        const auto store = [&](int r, int d, float v) {
+        // `v` of weight `all`, by reference `ref_of`
+        const auto store = [&](int r, int d, float v, float ref_of, float all) {
             if (d >= p.cache.dim) return;
-            v = row_sees[r] ? v : 0.f;
+            if (p.many == 2) {   // and what the row sees of the prefix, in parts
+                const int row = (seq * p.tokens) * group + row0 + r, tiles = (p.cache.seqs * rows + 255) / 256, tile = row / 256;
+                const float* const part = p.pre + ((int64_t)(head * tiles + tiles - 1 - tile) * p.splits * 256 + row % 256) * (kDim + 4);
+                float top = all > 0.f ? ref_of : kBottom;
+                for (int i = 0; i < p.splits; i++) {
+                    const float2 state = __ldcg((const float2*)(part + (int64_t)i * 256 * (kDim + 4) + kDim));
+                    if (state.y != 0.f) top = fmaxf(top, state.x);
+                }
+                const float f = all > 0.f ? exp2_fast(ref_of - top) : all == 0.f ? 0.f : 1.f;
+                v *= f, all *= f;
+                for (int i = 0; i < p.splits; i++) {
+                    const float* const at = part + (int64_t)i * 256 * (kDim + 4);
+                    const float2 state = __ldcg((const float2*)(at + kDim));
+                    if (state.y == 0.f) continue;
+                    const float g = exp2_fast(state.x - top);
+                    v += g * __ldcg(at + d), all += g * state.y;
+                }
+            }
+            v = row_sees[r] ? v / all : 0.f;
             if constexpr (F32Q) ((float*)p.out)[row_to[r] + d] = v;
             else ((__half*)p.out)[row_to[r] + d] = __float2half_rn(v);
         };
@@ -740,7 +759,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                 float v = 0.f;
 #pragma unroll
                 for (int w = 0; w < kWarps; w++) v += join[w * G::kRows * 32 + at];
-                if (whole) store(r, d, v / row_all[r]);
+                if (whole) store(r, d, v, most_of(r), row_all[r]);
                 else partial[r * kDim + d] = v;
             }
             __syncthreads();
@@ -790,10 +809,10 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                         all += f * state.y;
                         v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
                     }
-                    store(r, d, v.x / all);
-                    store(r, d + 1, v.y / all);
-                    store(r, d + 2, v.z / all);
-                    store(r, d + 3, v.w / all);
+                    store(r, d, v.x, m, all);
+                    store(r, d + 1, v.y, m, all);
+                    store(r, d + 2, v.z, m, all);
+                    store(r, d + 3, v.w, m, all);
                 }
             }
             __syncthreads();
@@ -849,6 +868,8 @@ CacheAttentionPlan cache_attention_plan(const CacheAttentionParams& p) {
 
 int launch_cache_attention(const CacheAttentionParams& p, cudaStream_t stream) {
     int err = 0;
+    if (p.many != 0) err = launch_cache_attention_rows(p, stream);
+    if (err != 0 || p.many == 1) return err;
     with_variant(p, [&](auto geo, auto kernel) {
         using G = decltype(geo);
         static bool done[64];

@@ -792,22 +792,39 @@ class Planner {
         }
         if (out.ss.size() == 0) return out;
         KN_CHECK((int64_t)p.tokens * p.heads * p.cache.seqs < (1ll << 31), KN_ERR_UNSUPPORTED, "cache attention: too many rows");
-        const CacheAttentionPlan plan = cache_attention_plan(p);
+        CacheAttentionPlan plan = cache_attention_plan(p);
+        // Many rows that share keys: 128 at a time on the tensor cores (i8 caches, whose values are finite whatever was written)
+        if (p.half && !p.cache.half && p.cache.dim <= 128) {
+            const int64_t group = p.heads / p.cache.heads, rows = p.tokens * group;
+            if (rows >= kManyRows) p.many = 1;
+            else if (p.prefix.dim && rows * p.cache.seqs >= kManyRows && p.prefix.capacity >= kManyKeys) p.many = 2;
+        }
+        if (p.many != 0) {
+            const CacheRowsPlan rows = cache_attention_rows_plan(p, p.many);
+            KN_CHECK(rows.items * rows.splits < (1ll << 31), KN_ERR_UNSUPPORTED, "cache attention: too many rows");
+            p.row_items = (int)rows.items, p.splits = rows.splits;
+            plan.part_floats = rows.part_floats;
+            if (p.many == 1) plan.units = plan.partial_floats = 0, plan.items = rows.items;
+            s.launches = p.many;
+        }
         KN_CHECK(plan.units < 2e9, KN_ERR_UNSUPPORTED, "cache attention: too much work for one step");
         p.grid = plan.grid;
-        if (plan.partial_floats) {
-            add(alloc_shared({plan.partial_floats}, DType::F32, v), 1);
+        s.optional.partial = plan.partial_floats || (p.many == 1 && p.splits > 1);
+        if (s.optional.partial) {
+            add(alloc_shared({std::max<int64_t>(plan.partial_floats, 1)}, DType::F32, v), 1);
             PlanTensor arrived = alloc_shared({plan.items}, DType::U32, v);
             buffer(arrived.buf).always_live = true;   // (zero between launches)
             add(arrived, 1);
         }
+        if (plan.part_floats) add(alloc_shared({plan.part_floats}, DType::F32, v), 1);
         s.optional.count = info.count_at >= 0, s.optional.slopes = info.slopes_at >= 0, s.optional.prefix = info.prefix_at >= 0;
         // what it needs where every sequence is as long as the cache
         const double keys = (double)p.cache.capacity + (p.prefix.dim ? p.prefix.capacity : 0);
         s.flops = 4.0 * p.cache.seqs * p.tokens * p.heads * p.cache.dim * keys;
         s.desc = "cacheattention seqs=" + std::to_string(p.cache.seqs) + " tokens=" + std::to_string(p.tokens) + " heads=" + std::to_string(p.heads) + "/" +
                  std::to_string(p.cache.heads) + " dim=" + std::to_string(p.cache.dim) + " capacity=" + std::to_string(p.cache.capacity) +
-                 (info.prefix_at >= 0 ? " prefix=" + std::to_string(p.prefix.capacity) : "") + (p.half ? " f16" : " f32") + " cache " + dtype_name(cache.dtype);
+                 (info.prefix_at >= 0 ? " prefix=" + std::to_string(p.prefix.capacity) : "") + (p.half ? " f16" : " f32") + " cache " + dtype_name(cache.dtype) +
+                 (p.many == 1 ? ", 128 rows at a time" : p.many == 2 ? ", the prefix 128 rows at a time" : "");
         push_step(std::move(s));
         return out;
     }

@@ -56,7 +56,7 @@ const char* step_kind_name(StepKind k);
 
 // Which of the operands that may be left out a step has
 struct OptionalOperands {
-    bool count = false, slopes = false, prefix = false;                       // CacheAttention
+    bool count = false, slopes = false, prefix = false, partial = false;     // CacheAttention
     bool temperature = false, top_k = false, top_p = false, min_p = false;   // Sample
 };
 

@@ -427,6 +427,77 @@ def test_attention_with_a_shared_prefix(dtype, prefix, length, own, tokens, more
     check_attention(3, tokens, 8, 2, 64, 60, own, dtype, prefix=prefix, prefix_length=length, **more)
 
 
+def plan_says(text, **sizes):
+    return text in plan_describe(attention_graph(**sizes), 1)
+
+
+def test_which_rows_are_taken_128_at_a_time():
+    assert plan_says(", 128 rows at a time", tokens=32, heads=4, kv_heads=2)
+    assert not plan_says("rows at a time", tokens=31, heads=4, kv_heads=2)
+    for no in (dict(dtype=F32), dict(storage=F16), dict(dim=136)):
+        assert not plan_says("rows at a time", tokens=100, heads=4, kv_heads=2, **no)
+    assert plan_says("the prefix 128 rows at a time", sequences=32, prefix=256)
+    assert not plan_says("rows at a time", sequences=31, prefix=256) and not plan_says("rows at a time", sequences=32, prefix=255)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [20, 64, 100, 128])
+@pytest.mark.parametrize("sequences, heads, kv_heads, tokens, capacity, start", [
+    (2, 4, 2, 32, 40, [8, 0]), (1, 1, 1, 128, 128, [0]), (1, 1, 1, 129, 200, [60]), (2, 8, 2, 70, 700, [600, 33]), (1, 2, 1, 300, 2100, [1790]), (3, 7, 1, 40, 64, [24, 0, 11])])
+def test_attention_of_many_rows(dim, sequences, heads, kv_heads, tokens, capacity, start):
+    assert plan_says(", 128 rows at a time", sequences=sequences, tokens=tokens, heads=heads, kv_heads=kv_heads, dim=dim, capacity=capacity)
+    check_attention(sequences, tokens, heads, kv_heads, dim, capacity, start)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("more", [dict(softcap=5.0), dict(window=1), dict(window=70), dict(slopes=True), dict(softcap=30.0, window=200, slopes=True), dict(prefix=90, prefix_length=77),
+                                  dict(prefix=500, window=130), dict(prefix=64, softcap=20.0, slopes=True), dict(prefix=300, prefix_length=0), dict(scale=-0.3)], ids=str)
+def test_attention_scores_of_many_rows(more):
+    check_attention(2, 80, 4, 2, 64, 450, [370, 9], **more)
+
+
+@pytest.mark.gpu
+def test_attention_of_padded_many_rows():
+    got = check_attention(6, 70, 4, 2, 64, 100, [5, -30, 60, -90, 2 ** 31 - 1, -2 ** 31], count=[40, 70, 70, 70, 70, 70])
+    assert (got[0, 40:] == 0).all() and (got[1, :30] == 0).all() and (got[3] == 0).all() and (got[5] == 0).all()
+    got = check_attention(2, 66, 4, 2, 64, 100, [150, 33], window=20)
+    assert (got[0] == 0).all() and (got[1] != 0).any(-1).all()
+    check_attention(3, 64, 2, 1, 128, 64, [0, 0, 0], count=[0, -3, 100])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", [np.inf, np.nan])
+def test_hidden_positions_of_many_rows_may_hold_anything(what):
+    heads, dim, capacity, tokens = 2, 64, 200, 64
+    cache, plain = filled(1, heads, capacity, dim, I8, 1)
+    g = Graph()
+    c = g.cache(1, heads, capacity, dim, I8)
+    k, start = g.input((1, 1, heads, dim)), g.input((1,), I32)
+    g.cache_write(c, k, k, start)
+    bad = np.full((1, 1, heads, dim), what, np.float32)
+    with CudaExecutor(0, g, 1) as ex:
+        ex.set_cache(0, cache)
+        for at in (170, 199, 20, 163):       # behind the end, in front of the window, the last new token
+            ex.evaluate([bad, np.array([at], np.int32)])
+    q = numbers(9, 1, tokens, heads, dim)
+    got = attend(attention_graph(1, tokens, heads, heads, dim, capacity, F16, I8, window=60), [cache], [q, np.array([100], np.int32)]).astype(np.float64)
+    want, size, sums = plain_attention(q[:, :63], plain.held, [100], window=60)
+    assert (np.abs(got[:, :63] - want).max(-1) <= attention_tolerance(F16, size, sums, capacity)).all()
+    assert np.isnan(got[:, 63]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sequences, heads, kv_heads, dim, tokens, prefix, length, more", [
+    (40, 8, 2, 128, 1, 1000, None, {}), (70, 4, 4, 64, 1, 256, 100, {}), (9, 8, 1, 100, 2, 300, 0, {}), (33, 4, 1, 128, 1, 4000, 3999, dict(window=300)),
+    (16, 16, 2, 64, 3, 700, 650, dict(slopes=True, softcap=15.0)), (70, 8, 1, 64, 1, 512, 512, {})])
+def test_prefix_of_all_sequences_at_once(sequences, heads, kv_heads, dim, tokens, prefix, length, more):
+    sizes = dict(sequences=sequences, tokens=tokens, heads=heads, kv_heads=kv_heads, dim=dim, capacity=60, prefix=prefix)
+    assert plan_says("the prefix 128 rows at a time", **sizes)
+    start = [(7 * s) % (60 - tokens) for s in range(sequences)]
+    start[1], start[2] = -1, -9                                     # sequences that see nothing (of their own, or at all)
+    check_attention(sequences, tokens, heads, kv_heads, dim, 60, start, prefix=prefix, prefix_length=length, count=[tokens] * (sequences - 1) + [0], **more)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_attention_of_padded_and_empty_rows(dtype):
