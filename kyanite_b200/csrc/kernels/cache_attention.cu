@@ -713,22 +713,25 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
         // `v` of weight `all`, by reference `ref_of`
         const auto store = [&](int r, int d, float v, float ref_of, float all) {
             if (d >= p.cache.dim) return;
-            if (p.many == 2) {   // and what the row sees of the prefix, in parts
+            if (p.many == 2) {   // and what the row sees of the prefix, in up to eight parts (of no sum where it sees nothing)
                 const int row = (seq * p.tokens) * group + row0 + r, tiles = (p.cache.seqs * rows + 255) / 256, tile = row / 256;
                 const float* const part = p.pre + ((int64_t)(head * tiles + tiles - 1 - tile) * p.splits * 256 + row % 256) * (kDim + 4);
-                float top = all > 0.f ? ref_of : kBottom;
-                for (int i = 0; i < p.splits; i++) {
-                    const float2 state = __ldcg((const float2*)(part + (int64_t)i * 256 * (kDim + 4) + kDim));
-                    if (state.y != 0.f) top = fmaxf(top, state.x);
+                float2 state[8];
+                float x[8], top = all > 0.f ? ref_of : kBottom;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float* const at = part + (int64_t)min(i, p.splits - 1) * 256 * (kDim + 4);
+                    state[i] = __ldcg((const float2*)(at + kDim));
+                    x[i] = __ldcg(at + d);
+                    if (i >= p.splits) state[i].y = 0.f;
+                    if (state[i].y != 0.f) top = fmaxf(top, state[i].x);
                 }
                 const float f = all > 0.f ? exp2_fast(ref_of - top) : all == 0.f ? 0.f : 1.f;
                 v *= f, all *= f;
-                for (int i = 0; i < p.splits; i++) {
-                    const float* const at = part + (int64_t)i * 256 * (kDim + 4);
-                    const float2 state = __ldcg((const float2*)(at + kDim));
-                    if (state.y == 0.f) continue;
-                    const float g = exp2_fast(state.x - top);
-                    v += g * __ldcg(at + d), all += g * state.y;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float g = exp2_fast(state[i].x - top);
+                    if (state[i].y != 0.f) v += g * x[i], all += g * state[i].y;
                 }
             }
             v = row_sees[r] ? v / all : 0.f;

@@ -13,7 +13,7 @@
 // their place and are the A operand of the second product, whose accumulator stays.  Scales of keys multiply scores, those of values
 // weights, in f32.  Weights go by a reference that no score is more than 2^8 above; it moves rarely, and then the thread rescales its
 // row (once the block before has been added).  Where the items are fewer than the SMs their keys are split over several
-// CTAs, the last of which joins the parts in order.
+// CTAs, and a second kernel joins the parts in order.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
     // q_full, then per stage full and empty, then per tile and parity of the block: scores complete, weights ready, values added
     const uint32_t q_full = bars, full = bars + 8, empty = full + 8 * kStages, s_full = empty + 8 * kStages, p_ready = s_full + 32, pv_done = p_ready + 32;
     __shared__ uint32_t tmem_slot;
-    __shared__ int abandon_flag, any_lo[2], any_hi[2], all_lo[2], all_hi[2], is_last;
+    __shared__ int abandon_flag, any_lo[2], any_hi[2], all_lo[2], all_hi[2];
     __shared__ float value_most[kStages][2];
     volatile int* const abandon = &abandon_flag;
     float* const scales = (float*)(gen + G::kScales);
@@ -418,47 +418,47 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
-    if (splits == 1 || prefix_only) return;
-    // ---------------- the last of an item's CTAs joins their parts
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const uint32_t before = atomicAdd(p.arrived + item, 1u);
-        is_last = before == (uint32_t)(splits - 1);
-        if (is_last) p.arrived[item] = 0;
-        __threadfence();
-    }
-    __syncthreads();
-    if (!is_last) return;
-    const float* const parts = p.pre + (int64_t)item * splits * kRows * (kDim + 4);
-    for (int i = threadIdx.x; i < min(kRows, rows - row0) * (kDim / 4); i += kThreads) {
-        const int r = i / (kDim / 4), d = i % (kDim / 4) * 4, t = token_of(row0 + r);
-        float most = kBottom, all = 0.f;
-        float4 v = make_float4(0, 0, 0, 0);
-        const auto part_of = [&](int k) { return parts + ((int64_t)k * kRows + r) * (kDim + 4); };
-#pragma unroll 4
-        for (int k = 0; k < splits; k++) {
-            const float2 state = __ldcg((const float2*)(part_of(k) + kDim));
-            if (state.y == 0.f) continue;   // (saw nothing, and may have written nothing)
-            most = fmaxf(most, state.x);
-        }
-#pragma unroll 4
-        for (int k = 0; k < splits; k++) {
-            const float2 state = __ldcg((const float2*)(part_of(k) + kDim));
-            if (state.y == 0.f) continue;
-            const float4 x = __ldcg((const float4*)(part_of(k) + d));
-            const float f = exp2_approx(state.x - most);
-            all += f * state.y;
-            v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
-        }
-        const int64_t at = (int64_t)p.start[item_seq] + t, last = min(at + shared, (int64_t)shared + p.cache.capacity - 1);
-        const bool sees = at >= 0 && (p.count == nullptr || t < p.count[item_seq]) && (p.window == 0 || last > at + shared - p.window);
-        const float x[4] = {v.x / all, v.y / all, v.z / all, v.w / all};
-        __half* const out = (__half*)p.out + (((int64_t)item_seq * p.tokens + t) * p.heads + head * group + (row0 + r) % group) * p.cache.dim;
+}
+
+// The parts of a row, a warp each
+template <int DB>
+__global__ void __launch_bounds__(256) cache_attention_join_kernel(const __grid_constant__ CacheAttentionParams p) {
+    constexpr int kDim = 64 * DB, kEach = kDim / 32;   // channels of a lane
+    pdl_enter();
+    const int group = p.heads / p.cache.heads, rows = p.tokens * group, row_tiles = (rows + kRows - 1) / kRows, lane = threadIdx.x & 31;
+    const int shared = p.prefix.base ? min(max(*p.prefix_length, 0), p.prefix.capacity) : 0;
+    const int64_t index = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);   // of all rows of all sequences and heads
+    if (index >= (int64_t)p.cache.seqs * p.cache.heads * rows) return;
+    const int row = (int)(index % rows), head = (int)(index / rows % p.cache.heads), seq = (int)(index / rows / p.cache.heads), t = row / group;
+    const int64_t item = ((int64_t)seq * p.cache.heads + head) * row_tiles + row_tiles - 1 - row / kRows;
+    const float* const part = p.pre + (item * p.splits * kRows + row % kRows) * (kDim + 4);
+    const int64_t step = (int64_t)kRows * (kDim + 4);
+    // (a part that saw nothing has no sum, and may have written no more than that)
+    const float2 mine = lane < p.splits ? __ldcg((const float2*)(part + lane * step + kDim)) : make_float2(kBottom, 0.f);
+    const float top = [&] {
+        float m = mine.y != 0.f ? mine.x : kBottom;
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        return m;
+    }();
+    const float factor = mine.y != 0.f ? exp2_approx(mine.x - top) : 0.f;
+    float all = mine.y != 0.f ? factor * mine.y : 0.f, v[kEach] = {};
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+#pragma unroll 8
+    for (int k = 0; k < p.splits; k++) {
+        const float f = __shfl_sync(0xffffffffu, factor, k);
+        const bool some = __shfl_sync(0xffffffffu, mine.y, k) != 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (d + k < p.cache.dim) out[d + k] = __float2half_rn(sees ? x[k] : 0.f);
+        for (int c = 0; c < kEach; c++) {
+            const float x = __ldcg(part + k * step + lane * kEach + c);
+            v[c] += some ? f * x : 0.f;
+        }
     }
+    const int64_t at = (int64_t)p.start[seq] + t, last = min(at + shared, (int64_t)shared + p.cache.capacity - 1);
+    const bool sees = at >= 0 && (p.count == nullptr || t < p.count[seq]) && (p.window == 0 || last > at + shared - p.window);
+    __half* const out = (__half*)p.out + (((int64_t)seq * p.tokens + t) * p.heads + head * group + row % group) * p.cache.dim + lane * kEach;
+#pragma unroll
+    for (int c = 0; c < kEach; c++)
+        if (lane * kEach + c < p.cache.dim) out[c] = __float2half_rn(sees ? v[c] / all : 0.f);
 }
 
 }  // namespace
@@ -469,8 +469,8 @@ CacheRowsPlan cache_attention_rows_plan(const CacheAttentionParams& p, int many)
     const int64_t rows = (int64_t)(many == 2 ? p.cache.seqs : 1) * p.tokens * (p.heads / p.cache.heads), dim = (p.cache.dim + 63) / 64 * 64;
     plan.items = (rows + kRows - 1) / kRows * p.cache.heads * (many == 2 ? 1 : p.cache.seqs);
     const int64_t blocks = (p.prefix.dim ? (p.prefix.capacity + kKeys - 1) / kKeys : 0) + (many == 2 ? 0 : (p.cache.capacity + kKeys - 1) / kKeys);
-    // parts of 8 blocks and more, for as many CTAs as there are SMs
-    plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({148 / plan.items, blocks / 8, 32}));
+    // parts of 8 blocks and more, for as many CTAs as there are SMs (of a prefix: as many as cache_attention_kernel takes)
+    plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({148 / plan.items, blocks / 8, many == 2 ? 8 : 32}));
     plan.part_floats = plan.splits > 1 || many == 2 ? plan.items * plan.splits * kRows * (dim + 4) : 0;
     return plan;
 }
@@ -485,6 +485,10 @@ int launch_cache_attention_rows(const CacheAttentionParams& p, cudaStream_t stre
     const dim3 grid((unsigned)(p.row_items * p.splits));
     if (blocks == 1) launch_pdl(cache_attention_rows_kernel<1>, grid, dim3(kThreads), RowsGeo<1>::kShared, stream, p);
     else launch_pdl(cache_attention_rows_kernel<2>, grid, dim3(kThreads), RowsGeo<2>::kShared, stream, p);
+    if (p.many == 1 && p.splits > 1) {
+        const int64_t rows = (int64_t)p.cache.seqs * p.tokens * p.heads;
+        launch_pdl(blocks == 1 ? cache_attention_join_kernel<1> : cache_attention_join_kernel<2>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, p);
+    }
     return (int)cudaGetLastError();
 }
 

@@ -804,14 +804,14 @@ class Planner {
             KN_CHECK(rows.items * rows.splits < (1ll << 31), KN_ERR_UNSUPPORTED, "cache attention: too many rows");
             p.row_items = (int)rows.items, p.splits = rows.splits;
             plan.part_floats = rows.part_floats;
-            if (p.many == 1) plan.units = plan.partial_floats = 0, plan.items = rows.items;
-            s.launches = p.many;
+            if (p.many == 1) plan.units = plan.partial_floats = 0;
+            s.launches = p.many == 2 || rows.splits > 1 ? 2 : 1;
         }
         KN_CHECK(plan.units < 2e9, KN_ERR_UNSUPPORTED, "cache attention: too much work for one step");
         p.grid = plan.grid;
-        s.optional.partial = plan.partial_floats || (p.many == 1 && p.splits > 1);
+        s.optional.partial = plan.partial_floats != 0;
         if (s.optional.partial) {
-            add(alloc_shared({std::max<int64_t>(plan.partial_floats, 1)}, DType::F32, v), 1);
+            add(alloc_shared({plan.partial_floats}, DType::F32, v), 1);
             PlanTensor arrived = alloc_shared({plan.items}, DType::U32, v);
             buffer(arrived.buf).always_live = true;   // (zero between launches)
             add(arrived, 1);
