@@ -65,6 +65,23 @@ __device__ __forceinline__ void mma_f16_weights(uint32_t tmem_d, uint32_t tmem_a
 }
 __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
+// Two products, or sums, in one instruction
+__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*(uint64_t*)&a), "l"(*(uint64_t*)&b));
+    return *(float2*)&d;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*(uint64_t*)&a), "l"(*(uint64_t*)&b));
+    return *(float2*)&d;
+}
+__device__ __forceinline__ float max_of(float a, float b, float c) {   // (of numbers: a NaN is passed over)
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // What a row sees, in positions of a run (0: the prefix, 1: its sequence's own)
 struct Sight {
     int low[2], high[2];
@@ -167,57 +184,62 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
         const float log2e = 1.4426950408889634f;
         const float unit = p.softcap > 0.f ? p.scale * 2.f * log2e / p.softcap : p.scale * log2e;
         constexpr int kAcross = kDim / 16;
-        uint4 now[G::kChunks], next[G::kChunks];
-        float scale_now = 0.f, scale_next = 0.f;
-        const auto load = [&](int j, uint4 (&raw)[G::kChunks], float& scale) {
+        // piece i of this thread: of part i / (pieces of a part), of key i x kApart + key_of_mine in it, always the same 16 channels
+        constexpr int kApart = 128 / kAcross, kOfPart = G::kChunks / 2;
+        const int my_key = me / kAcross, chunk = me % kAcross;   // (kApart is a multiple of 16: the order in a row is the key's)
+        const int from_at = (my_key & 15) * G::kRowBytes + ((chunk ^ cache_swizzle(G::kRowBytes, my_key & 15)) << 4);
+        const int to_at = (chunk >> 2) * (kKeys * 128) + my_key * 128, to_lo = (((chunk & 3) * 2) ^ (my_key & 7)) << 4, to_hi = (((chunk & 3) * 2 + 1) ^ (my_key & 7)) << 4;
+        struct Block {
+            uint4 raw[G::kChunks];
+            float scale;
+        };
+        const auto load = [&](int j, Block& b) {
             const int run = from + j >= n0, kb = run ? first1 + from + j - n0 : first0 + from + j;
             const CacheParams& c = run ? p.cache : p.prefix;
             const uint8_t* const head_at = c.base + ((run ? (int64_t)item_seq * c.heads : 0) + head) * ((int64_t)c.tiles * c.tile_bytes);
+            const uint8_t* const at = head_at + (int64_t)(kb * (kKeys / kCacheTile)) * c.tile_bytes + from_at;
+            const int last = c.tiles - 1 - kb * (kKeys / kCacheTile);   // (behind it: any numbers will do, nobody sees them)
 #pragma unroll
             for (int i = 0; i < G::kChunks; i++) {
-                const int x = i * 128 + me, part = x / (kKeys * kAcross), key = x / kAcross % kKeys, chunk = x % kAcross;
-                const int tile = kb * (kKeys / kCacheTile) + (key >> 4);
-                raw[i] = make_uint4(kCacheZeros, kCacheZeros, kCacheZeros, kCacheZeros);
-                if (tile < c.tiles)
-                    raw[i] = __ldcg((const uint4*)(head_at + (int64_t)tile * c.tile_bytes + (part * kCacheTile + (key & 15)) * G::kRowBytes + ((chunk ^ cache_swizzle(G::kRowBytes, key & 15)) << 4)));
+                const int part = i / kOfPart, tile = (i % kOfPart * kApart + my_key) >> 4;
+                b.raw[i] = __ldcg((const uint4*)(at + min(tile, last) * c.tile_bytes + part * kCacheTile * G::kRowBytes));
             }
             // a scale a thread: of keys, then of values; what no row sees has none
             const int part = me >> 6, key = kb * kKeys + (me & 63);
-            scale = 0.f;
+            b.scale = 0.f;
             if (key >= any_lo[run] && key < any_hi[run])
-                scale = __ldcg((const float*)(head_at + (int64_t)(key >> 4) * c.tile_bytes + 2 * kCacheTile * G::kRowBytes) + part * kCacheTile + (key & 15));
-            if (part == 0) scale *= unit;
+                b.scale = __ldcg((const float*)(head_at + (int64_t)(key >> 4) * c.tile_bytes + 2 * kCacheTile * G::kRowBytes) + part * kCacheTile + (key & 15));
+            if (part == 0) b.scale *= unit;
         };
-        if (n > 0) load(0, now, scale_now);
-        for (int j = 0; j < n; j++) {
+        const auto step = [&](int j, Block& now, Block& next) -> bool {
             const int st = j % kStages;
-            if (j + 1 < n) load(j + 1, next, scale_next);
+            if (j + 1 < n) load(j + 1, next);
             bool good = true;
             if (j >= kStages) good = mbar_wait(empty + 8 * st, (uint32_t)((j / kStages - 1) & 1), abandon, p.status, 81, kWaitCycles, kSleepNs);
-            if (!__all_sync(0xffffffffu, good)) break;
-            uint8_t* const to = gen + 2 * G::kQTile + st * G::kStage;
+            if (!__all_sync(0xffffffffu, good)) return false;
+            uint8_t* const to = gen + 2 * G::kQTile + st * G::kStage + to_at;
 #pragma unroll
             for (int i = 0; i < G::kChunks; i++) {
-                const int x = i * 128 + me, part = x / (kKeys * kAcross), key = x / kAcross % kKeys, chunk = x % kAcross;
-                const uint32_t w[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
-                uint8_t* const at = to + part * G::kPart + (chunk >> 2) * (kKeys * 128) + key * 128;
-                const int c0 = (chunk & 3) * 2;
-                *(uint4*)(at + ((c0 ^ (key & 7)) << 4)) = make_uint4(two_low(w[0]), two_high(w[0]), two_low(w[1]), two_high(w[1]));
-                *(uint4*)(at + (((c0 + 1) ^ (key & 7)) << 4)) = make_uint4(two_low(w[2]), two_high(w[2]), two_low(w[3]), two_high(w[3]));
+                uint8_t* const at = to + i / kOfPart * G::kPart + i % kOfPart * kApart * 128;
+                const uint4 w = now.raw[i];
+                *(uint4*)(at + to_lo) = make_uint4(two_low(w.x), two_high(w.x), two_low(w.y), two_high(w.y));
+                *(uint4*)(at + to_hi) = make_uint4(two_low(w.z), two_high(w.z), two_low(w.w), two_high(w.w));
             }
-            scales[(st * 2 + (me >> 6)) * kKeys + (me & 63)] = scale_now;
+            scales[(st * 2 + (me >> 6)) * kKeys + (me & 63)] = now.scale;
             if (me >= 64) {
-                float most = scale_now;
+                float most = now.scale;
                 for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                 if (lane == 0) value_most[st][warp & 1] = most;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) arrive(full + 8 * st);
-#pragma unroll
-            for (int i = 0; i < G::kChunks; i++) now[i] = next[i];
-            scale_now = scale_next;
-        }
+            return true;
+        };
+        Block one, two;
+        if (n > 0) load(0, one);
+        for (int j = 0; j < n; j += 2)
+            if (!step(j, one, two) || (j + 1 < n && !step(j + 1, two, one))) break;
     } else if (warp == 12) {
         if (elect_one() && n > 0) {
             // ---------------- MMA issuer (see kernels/flash.cu)
@@ -291,33 +313,37 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             const float4* const ks = (const float4*)(scales + st * 2 * kKeys);
             const float4* const vs = ks + kKeys / 4;
-            float top = -INFINITY;
+            float2 x[32];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const float4 k = ks[i];
-                const float f[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-                for (int c = 0; c < 4; c++) v[i >> 3][(4 * i + c) & 31] = __float_as_uint(__uint_as_float(v[i >> 3][(4 * i + c) & 31]) * f[c]);
+                const int c = 4 * i & 31;
+                x[2 * i] = mul_pair(make_float2(__uint_as_float(v[i >> 3][c]), __uint_as_float(v[i >> 3][c + 1])), make_float2(k.x, k.y));
+                x[2 * i + 1] = mul_pair(make_float2(__uint_as_float(v[i >> 3][c + 2]), __uint_as_float(v[i >> 3][c + 3])), make_float2(k.z, k.w));
             }
             if (p.softcap > 0.f) {
+                const auto capped = [&](float y) { return cap - __fdividef(2.f * cap, 1.f + exp2_approx(fminf(y, 126.f))); };   // tanh(y) = 1 - 2 / (1 + e^(2y))
 #pragma unroll
-                for (int i = 0; i < 64; i++)   // tanh(y) = 1 - 2 / (1 + e^(2y))
-                    v[i >> 5][i & 31] = __float_as_uint(cap - __fdividef(2.f * cap, 1.f + exp2_approx(fminf(__uint_as_float(v[i >> 5][i & 31]), 126.f))));
+                for (int i = 0; i < 32; i++) x[i] = make_float2(capped(x[i].x), capped(x[i].y));
             }
             if (p.slopes) {
                 const float away = (float)(position + (run ? 0 : shared) - key0);
 #pragma unroll
-                for (int i = 0; i < 64; i++) v[i >> 5][i & 31] = __float_as_uint(__uint_as_float(v[i >> 5][i & 31]) - slope * (away - (float)i));
+                for (int i = 0; i < 32; i++) x[i].x -= slope * (away - (float)(2 * i)), x[i].y -= slope * (away - (float)(2 * i + 1));
             }
             const bool masked = key0 < all_lo[run] || key0 + kKeys > all_hi[run];   // some row does not see all of it
+            const int lo = sight.low[run] - key0, hi = sight.live ? sight.high[run] - key0 : 0;
             if (masked) {
-                const int lo = sight.low[run] - key0, hi = sight.live ? sight.high[run] - key0 : 0;
 #pragma unroll
-                for (int i = 0; i < 64; i++)
-                    if (i < lo || i >= hi) v[i >> 5][i & 31] = 0xff800000u;
+                for (int i = 0; i < 32; i++) {
+                    if (2 * i < lo || 2 * i >= hi) x[i].x = -INFINITY;
+                    if (2 * i + 1 < lo || 2 * i + 1 >= hi) x[i].y = -INFINITY;
+                }
             }
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 64; i++) top = fmaxf(top, __uint_as_float(v[i >> 5][i & 31]));
+            for (int i = 0; i < 32; i++) tops[i & 3] = max_of(tops[i & 3], x[i].x, x[i].y);
+            const float top = max_of(fmaxf(tops[0], tops[1]), tops[2], tops[3]);
             // ---- the reference
             const float value_top = fmaxf(value_most[st][0], value_most[st][1]);
             const bool wider = value_top > value_ref || value_ref == 0.f;
@@ -339,31 +365,42 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
                 if (j > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
                     if (!wait(my_pv_done + 8 * ((j - 1) & 1), (uint32_t)(((j - 1) >> 1) & 1), 87)) { ok = false; break; }
 #pragma unroll 1
-                    for (int c = 0; c < kDim / 32; c++) {
-                        uint32_t o[32];
-                        tmem_load_32(my_o + c * 32, o);
+                    for (int c = 0; c < kDim / 16; c++) {
+                        uint32_t o[16];
+                        tmem_load_16_nowait(my_o + c * 16, o);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                        tmem_store_32(my_o + c * 32, o);
+                        for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                        tmem_store_16(my_o + c * 16, o);
                     }
                 }
             }
-            // ---- weights
+            // ---- weights.  (One that is hidden is 0, whatever its position's scale: 0 times a scale that is none is a NaN)
+            const float2 down = make_float2(-reference, -reference);
+            float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                const float2 y = add_pair(x[i], down);
+                x[i] = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                sums[i & 1] = add_pair(sums[i & 1], x[i]);
+            }
+            sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const float4 scale = vs[i];
-                float w[4];
+                const float4 f = vs[i];
+                x[2 * i] = mul_pair(x[2 * i], make_float2(f.x, f.y)), x[2 * i + 1] = mul_pair(x[2 * i + 1], make_float2(f.z, f.w));
+            }
+            if (masked) {
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    w[c] = exp2_approx(__uint_as_float(v[i >> 3][(4 * i + c) & 31]) - reference);
-                    sum += w[c];
+                for (int i = 0; i < 32; i++) {
+                    if (2 * i < lo || 2 * i >= hi) x[i].x = 0.f;
+                    if (2 * i + 1 < lo || 2 * i + 1 >= hi) x[i].y = 0.f;
                 }
-                // (a position that is hidden weighs 0, whatever its scale: 0 times a scale that is none is a NaN)
-                const float f[4] = {scale.x, scale.y, scale.z, scale.w};
+            }
 #pragma unroll
-                for (int c = 0; c < 4; c++) w[c] = masked && w[c] == 0.f ? 0.f : w[c] * f[c];
-                const __half2 lo = __floats2half2_rn(w[0], w[1]), hi = __floats2half2_rn(w[2], w[3]);
-                v[0][2 * i] = *(const uint32_t*)&lo, v[0][2 * i + 1] = *(const uint32_t*)&hi;
+            for (int i = 0; i < 32; i++) {
+                const __half2 h = __floats2half2_rn(x[i].x, x[i].y);
+                v[0][i] = *(const uint32_t*)&h;
             }
             tmem_store_32(my_s, v[0]);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
