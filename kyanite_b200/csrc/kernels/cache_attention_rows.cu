@@ -4,9 +4,9 @@
 //
 // A CTA has 256 rows, two accumulator tiles of 128, and takes 64 keys at a time:
 //
-//   warps 0..7      softmax: a row per thread, four warps a tile; the two tiles' exponentials run beside each other's products
+//   warps 0..7      queries once; softmax: a row per thread, four warps a tile; the two tiles' exponentials run beside each other's products
 //   warps 8..11     keys and values of 8 bits -> f16 in shared memory (exact; kernels/cache.cuh), three blocks of both in turn; their
-//                   scales; queries once
+//                   scales
 //   warp 12, a lane MMA issuer: the next block's scores go ahead of this block's products with the values, tile by tile
 //
 // Scores of a block are one of a tile's two accumulators of 64 columns in tensor memory; its weights, rounded to f16 and packed, take
@@ -96,8 +96,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* const gen = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t bars = base + G::kBars;
-    // q_full, then per stage full and empty, then per tile and parity of the block: scores complete, weights ready, values added
-    const uint32_t q_full = bars, full = bars + 8, empty = full + 8 * kStages, s_full = empty + 8 * kStages, p_ready = s_full + 32, pv_done = p_ready + 32;
+    // per tile: queries are there; per stage full and empty, then per tile and parity of the block: scores complete, weights ready, values added
+    const uint32_t q_full = bars, full = bars + 16, empty = full + 8 * kStages, s_full = empty + 8 * kStages, p_ready = s_full + 32, pv_done = p_ready + 32;
     __shared__ uint32_t tmem_slot;
     __shared__ int abandon_flag, any_lo[2], any_hi[2], all_lo[2], all_hi[2];
     __shared__ float value_most[kStages][2];
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
     float* const scales = (float*)(gen + G::kScales);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 4);
+        mbar_init(q_full, 4), mbar_init(q_full + 8, 4);
         for (int i = 0; i < kStages; i++) mbar_init(full + 8 * i, 4), mbar_init(empty + 8 * i, 1);
         for (int i = 0; i < 4; i++) mbar_init(s_full + 8 * i, 1), mbar_init(p_ready + 8 * i, 4), mbar_init(pv_done + 8 * i, 1);
         abandon_flag = 0;
@@ -140,11 +140,15 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
         sight.low[1] = p.window > 0 ? max(cut(position - p.window + 1), 0) : 0;
     }
     __syncthreads();   // (before the range is agreed on)
-    if (sight.live)
+    if (warp < 8) {
+#pragma unroll
         for (int r = 0; r < 2; r++) {
-            if (sight.low[r] < sight.high[r]) atomicMin(&any_lo[r], sight.low[r]), atomicMax(&any_hi[r], sight.high[r]);
-            atomicMax(&all_lo[r], sight.low[r]), atomicMin(&all_hi[r], sight.high[r]);
+            const bool some = sight.live && sight.low[r] < sight.high[r];
+            const int lo = __reduce_min_sync(0xffffffffu, some ? sight.low[r] : 1 << 30), hi = __reduce_max_sync(0xffffffffu, some ? sight.high[r] : -(1 << 30));
+            const int high_lo = __reduce_max_sync(0xffffffffu, sight.live ? sight.low[r] : -(1 << 30)), low_hi = __reduce_min_sync(0xffffffffu, sight.live ? sight.high[r] : 1 << 30);
+            if (lane == 0) atomicMin(&any_lo[r], lo), atomicMax(&any_hi[r], hi), atomicMax(&all_lo[r], high_lo), atomicMin(&all_hi[r], low_hi);
         }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -156,31 +160,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
     const int tiles = rows - row0 > kTileRows ? 2 : 1;
 
     if (warp >= 8 && warp < 12) {
-        // ---------------- queries, keys and values
+        // ---------------- keys and values
         const int me = threadIdx.x - 256;
-        if (n > 0) {
-            constexpr int kUnits = kDim / 8;   // 16 bytes of a row
-            for (int i = me; i < tiles * kTileRows * kUnits; i += 128) {
-                const int r = i / kUnits, unit = i % kUnits, d = unit * 8, q_row = row0 + r;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (q_row < rows && d < p.cache.dim) {
-                    const __half* at = (const __half*)p.query + (int64_t)seq_of(q_row) * p.q_strides[0] + (int64_t)token_of(q_row) * p.q_strides[1] +
-                                       (int64_t)(head * group + q_row % group) * p.q_strides[2];
-                    if (p.q_wide) {
-                        v = *(const uint4*)(at + d);
-                    } else {
-                        __half h[8];
-#pragma unroll
-                        for (int k = 0; k < 8; k++) h[k] = d + k < p.cache.dim ? at[(d + k) * p.q_strides[3]] : __half(0.f);
-                        v = *(const uint4*)h;
-                    }
-                }
-                *(uint4*)(gen + (r / kTileRows) * G::kQTile + (unit >> 3) * (kTileRows * 128) + (r % kTileRows) * 128 + (((unit & 7) ^ (r & 7)) << 4)) = v;
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) arrive(q_full);
-        }
         const float log2e = 1.4426950408889634f;
         const float unit = p.softcap > 0.f ? p.scale * 2.f * log2e / p.softcap : p.scale * log2e;
         constexpr int kAcross = kDim / 16;
@@ -263,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
                 }
                 return true;
             };
-            bool ok = mbar_wait(q_full, 0, abandon, p.status, 84, kWaitCycles, kSleepNs) && scores(0);
+            bool ok = mbar_wait(q_full, 0, abandon, p.status, 84, kWaitCycles, kSleepNs) && (tiles == 1 || mbar_wait(q_full + 8, 0, abandon, p.status, 84, kWaitCycles, kSleepNs)) && scores(0);
             for (int j = 0; j < n && ok; j++) {
                 const int st = j % kStages, b = j & 1;
                 if (j + 1 < n && !scores(j + 1)) break;   // under this block's exponentials
@@ -295,6 +276,31 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
             return good != 0;
         };
         const bool used = tile < tiles && n > 0;
+        // queries: of the warp's 32 rows, 16 bytes a lane
+        if (used) {
+            constexpr int kUnits = kDim / 8, kAtOnce = 32 / kUnits;   // units of 16 bytes of a row; rows of an access
+#pragma unroll 8
+            for (int i = 0; i < 32 / kAtOnce; i++) {
+                const int r = (threadIdx.x & (kRows - 1) & ~31) + i * kAtOnce + lane / kUnits, unit = lane % kUnits, d = unit * 8, q_row = row0 + r;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (q_row < rows && d < p.cache.dim) {
+                    const __half* at = (const __half*)p.query + (int64_t)seq_of(q_row) * p.q_strides[0] + (int64_t)token_of(q_row) * p.q_strides[1] +
+                                       (int64_t)(head * group + q_row % group) * p.q_strides[2];
+                    if (p.q_wide) {
+                        v = *(const uint4*)(at + d);
+                    } else {
+                        __half h[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) h[k] = d + k < p.cache.dim ? at[(d + k) * p.q_strides[3]] : __half(0.f);
+                        v = *(const uint4*)h;
+                    }
+                }
+                *(uint4*)(gen + tile * G::kQTile + (unit >> 3) * (kTileRows * 128) + (r % kTileRows) * 128 + (((unit & 7) ^ (r & 7)) << 4)) = v;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) arrive(q_full + 8 * tile);
+        }
         const float log2e = 1.4426950408889634f, cap = p.softcap * log2e;
         const float slope = p.slopes && row < rows ? p.slopes[head * group + row % group] * log2e : 0.f;
         // weights are 2^(x - reference): what the reference is above is 2^7 times a weight over the values' scale, so that weights times
