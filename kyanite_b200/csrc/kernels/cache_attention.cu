@@ -50,7 +50,9 @@ struct Geo {
     static constexpr int kBlocks = kDim / (8 * kE);
     static constexpr int kGroups = kRowBytes / 64;           // 64-byte groups of a key row: one 16-byte chunk a lane
     static constexpr int kSteps = HALF ? 2 : 4;              // products of 16 channels in one
-    static constexpr int kJoin = kWarps * kRows * 32;        // floats: what the warps exchange at a time, 32 channels
+    // floats: what the warps exchange at a time, 32 channels of all rows, or 128 where two stages leave room
+    static constexpr int kJoinTimes = kPerSm == 1 && kRowBytes >= 256 && kRowBytes != 384 && COLS == 2 ? 4 : 1;
+    static constexpr int kJoin = kWarps * kRows * 32 * kJoinTimes;
     static constexpr int kRoom = (220 * 1024 / kPerSm - kJoin * 4) / (kWarps * kStage);
     static constexpr int kStages = kRoom < 4 ? kRoom : 4;
     static constexpr int kShared = kWarps * kStages * kStage + kJoin * 4;
@@ -186,50 +188,65 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
         }
         __syncthreads();
     };
-    const auto all_of = [](int n) { return n; };
-    int total = 0;   // units
-    if (p.cache.seqs <= 64) {   // (every warp for itself)
-        int mine = (lane < p.cache.seqs ? units_at(lane) : 0) + (lane + 32 < p.cache.seqs ? units_at(lane + 32) : 0);
-        total = __reduce_add_sync(0xffffffffu, mine) * items;
-    } else {
-        for (int i = 0; i * kThreads < p.cache.seqs; i++) {
-            int mine;
-            scan(i, mine, all_of);
-            for (int w = 0; w < kWarps; w++) total += scan_sum[w];
-        }
-    }
     const int grid = gridDim.x;
-    // Items in whole parts of up to `most` units, one part per CTA, where that is hardly longer than equal ranges: a CTA does not change
-    // items then.  (A change and a join are about as long as two units.)
-    int most = 0;
-    if (p.cache.seqs <= 64) {
-        const int lane_units[2] = {lane < p.cache.seqs ? units_at(lane) : 0, lane + 32 < p.cache.seqs ? units_at(lane + 32) : 0};
+    int total = 0, most = 0;   // units; in a part, see below
+    const bool few = p.cache.seqs <= 64;   // every warp for itself then, two sequences a lane
+    int mine[2] = {0, 0};
+    if (few) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (2 * lane + i < p.cache.seqs) mine[i] = units_at(2 * lane + i);
+        total = __reduce_add_sync(0xffffffffu, mine[0] + mine[1]) * items;
+        // Items in whole parts of up to `most` units, one part per CTA, where that is hardly longer than equal ranges: a CTA does not change
+        // items then.  (A change and a join are about as long as two units.)
         const int least = (total + grid - 1) / grid;
         for (int q = least; q <= least + 2 && most == 0; q++)
-            if (__reduce_add_sync(0xffffffffu, (lane_units[0] + q - 1) / q + (lane_units[1] + q - 1) / q) * items <= grid) most = q;
+            if (__reduce_add_sync(0xffffffffu, (mine[0] + q - 1) / q + (mine[1] + q - 1) / q) * items <= grid) most = q;
+    } else {
+        for (int i = 0; i * kThreads < p.cache.seqs; i++) {
+            int one;
+            scan(i, one, [](int n) { return n; });
+            for (int w = 0; w < kWarps; w++) total += scan_sum[w];
+        }
     }
     // in equal ranges the first `longer` CTAs have one unit more
     const int ctas = min(grid, total), each = total / ctas, longer = total - each * ctas;
     const auto cta_of = [&](int u) { return u < longer * (each + 1) ? u / (each + 1) : longer + (u - longer * (each + 1)) / each; };
     const auto start_of = [&](int b) { return b * each + min(b, longer); };
-    int first_seq, first_item, first_from, todo, part = 0;
     const int u0 = start_of(blockIdx.x);   // (equal ranges)
-    if (most > 0) {
-        find(blockIdx.x, [&](int n) { return (n + most - 1) / most; });
-        first_seq = scan_seq;
-        if (first_seq < 0) return;
-        const int units = units_at(first_seq), parts = (units + most - 1) / most, at = blockIdx.x - scan_at;
-        first_item = at / parts;
-        part = at % parts;
-        first_from = (int)((int64_t)units * part / parts);
-        todo = (int)((int64_t)units * (part + 1) / parts) - first_from;
+    if (most == 0 && (int)blockIdx.x >= ctas) return;
+    int first_seq, first_units, place;   // where the CTA begins: its place among the units (or parts) of that sequence
+    if (few) {
+        const auto parts_of = [&](int n) { return (most > 0 ? (n + most - 1) / most : n) * items; };
+        const int x = most > 0 ? (int)blockIdx.x : u0, a = parts_of(mine[0]), b = parts_of(mine[1]);
+        int front = a + b;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int w = __shfl_up_sync(0xffffffffu, front, o);
+            if (lane >= o) front += w;
+        }
+        front -= a + b;
+        const uint32_t hit = __ballot_sync(0xffffffffu, front <= x && x < front + a + b);
+        if (hit == 0) return;
+        const int from = __ffs(hit) - 1, second = x >= front + a ? 1 : 0;
+        first_seq = __shfl_sync(0xffffffffu, 2 * lane + second, from);
+        first_units = __shfl_sync(0xffffffffu, mine[second], from);
+        place = __shfl_sync(0xffffffffu, x - front - (second ? a : 0), from);
     } else {
-        if ((int)blockIdx.x >= ctas) return;
-        find(u0, all_of);
+        find(u0, [](int n) { return n; });
         first_seq = scan_seq;
-        const int units = units_at(first_seq);
-        first_item = (u0 - scan_at) / units;
-        first_from = (u0 - scan_at) % units;
+        first_units = units_at(first_seq);
+        place = u0 - scan_at;
+    }
+    int first_item, first_from, todo, part = 0;
+    if (most > 0) {
+        const int parts = (first_units + most - 1) / most;
+        first_item = place / parts;
+        part = place % parts;
+        first_from = (int)((int64_t)first_units * part / parts);
+        todo = (int)((int64_t)first_units * (part + 1) / parts) - first_from;
+    } else {
+        first_item = place / first_units;
+        first_from = place % first_units;
         todo = each + ((int)blockIdx.x < longer ? 1 : 0);
     }
     int issued = 0, consumed = 0;
@@ -741,10 +758,10 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
         // 32 of a block's channels (four of each lane's) of all rows, or more of them of fewer rows, at a time
         constexpr int kPieces = G::kBlocks * kE / 4;
         const int row_bits = rows_here <= 1 ? 0 : rows_here <= 2 ? 1 : rows_here <= 4 ? 2 : rows_here <= 8 ? 3 : 4;
-        const int at_once = G::kRows >> row_bits;   // pieces
+        const int at_once = min((G::kRows >> row_bits) * G::kJoinTimes, kPieces);   // pieces (all powers of two, or all there are)
 #pragma unroll
         for (int piece = 0; piece < kPieces; piece++) {
-            const int b = piece / (kE / 4), i0 = piece % (kE / 4) * 2, place = piece & (at_once - 1);
+            const int b = piece / (kE / 4), i0 = piece % (kE / 4) * 2, place = piece % at_once;
 #pragma unroll
             for (int n = 0; n < COLS; n++)
 #pragma unroll
@@ -761,7 +778,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                 const int d = which / (kE / 4) * 8 * kE + kE * ((at & 31) >> 2) + which % (kE / 4) * 4 + (at & 3);
                 float v = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWarps; w++) v += join[w * G::kRows * 32 + at];
+                for (int w = 0; w < kWarps; w++) v += join[((w * at_once) << (row_bits + 5)) + at];
                 if (whole) store(r, d, v, most_of(r), row_all[r]);
                 else partial[r * kDim + d] = v;
             }
@@ -784,9 +801,9 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                 parts = cta_of(item_u + units - 1) - c0 + 1;
                 second = start_of(c0) < item_u;
             }
-            __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
+                __threadfence();   // (of all that the CTA has written: the barrier came first)
                 uint32_t* arrived = p.arrived + (int64_t)seq * items + item;
                 const uint32_t before = atomicAdd(arrived, 1u);
                 is_last = before == (uint32_t)(parts - 1);
@@ -801,16 +818,27 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                 for (int at = threadIdx.x; at < rows_here * kDim / 4; at += kThreads) {
                     const int r = at / (kDim / 4), d = at % (kDim / 4) * 4;
                     float m = kBottom, all = 0.f;
-#pragma unroll 8
-                    for (int i = 0; i < parts; i++) m = fmaxf(m, __ldcg(part_of(i) + G::kRows * kDim + 2 * r));
                     float4 v = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-                    for (int i = 0; i < parts; i++) {
-                        const float2 state = __ldcg((const float2*)(part_of(i) + G::kRows * kDim + 2 * r));
-                        const float4 x = __ldcg((const float4*)(part_of(i) + r * kDim + d));
-                        const float f = exp2_fast(state.x - m);
-                        all += f * state.y;
-                        v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
+                    for (int i0 = 0; i0 < parts; i0 += 8) {   // eight parts' loads in flight
+                        float2 state[8];
+                        float4 x[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float* const at_part = part_of(min(i0 + i, parts - 1));
+                            state[i] = __ldcg((const float2*)(at_part + G::kRows * kDim + 2 * r));
+                            x[i] = __ldcg((const float4*)(at_part + r * kDim + d));
+                        }
+                        float top = m;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) top = fmaxf(top, state[i].x);
+                        const float keep = exp2_fast(m - top);
+                        m = top;
+                        all *= keep, v.x *= keep, v.y *= keep, v.z *= keep, v.w *= keep;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float f = i0 + i < parts ? exp2_fast(state[i].x - m) : 0.f;
+                            if (i0 + i < parts) all += f * state[i].y, v.x += f * x[i].x, v.y += f * x[i].y, v.z += f * x[i].z, v.w += f * x[i].w;
+                        }
                     }
                     store(r, d, v.x, m, all);
                     store(r, d + 1, v.y, m, all);
