@@ -130,6 +130,7 @@ struct Executor {
     int launches = 0;                            // of one run of all steps
     std::vector<DenseChainParams> dense_runs;    // of plan->dense_runs
     std::vector<std::shared_ptr<CacheStorage>> caches;   // of plan->caches; null until attached
+    std::vector<uint8_t> cache_used;             // ... by a step
     Comm* comm = nullptr;              // not owned; AllReduce steps sum over its ranks (null: a world of one)
 
     ~Executor() {
@@ -168,6 +169,7 @@ struct Executor {
     // of them comes first.  (Nothing to do while one executor uses them.)
     void enter_caches() {
         for (size_t i = 0; i < caches.size(); i++) {
+            if (!cache_used[i]) continue;
             KN_CHECK(caches[i] != nullptr, KN_ERR_INVALID_ARG, "no cache is attached as cache " + std::to_string(i) + " (kn_executor_set_cache)");
             CacheStorage& c = *caches[i];
             std::lock_guard<std::mutex> lock(c.mu);
@@ -776,6 +778,10 @@ static std::unique_ptr<Executor> create_executor(int device, const Graph& graph,
         ex->dtype_out.push_back(plan.outputs[i].dtype);
     }
     ex->caches.resize(plan.caches.size());
+    ex->cache_used.resize(plan.caches.size());
+    for (const Step& s : plan.steps)
+        for (const PlanTensor& t : s.operands)
+            if (plan.buffers[t.buf].kind == BufKind::Cache) ex->cache_used[plan.buffers[t.buf].cache] = 1;
     KN_CUDA(cudaMemsetAsync(ex->arena, 0, std::max<size_t>(plan.arena_bytes, 256), ex->stream));
     ex->patch_pointers();
     KN_CUDA(cudaStreamSynchronize(ex->stream));

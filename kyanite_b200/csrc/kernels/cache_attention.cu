@@ -497,7 +497,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
 #pragma unroll
                     for (int n = 0; n < COLS; n++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) s[n][i] -= slope[n][i & 1] * ((float)(zero + t_of[n][i & 1]) - (float)(at + token[i >> 1]));
+                        for (int i = 0; i < 4; i++) s[n][i] -= slope[n][i & 1] * (float)((int)(zero + t_of[n][i & 1] - at) - token[i >> 1]);   // (positions may be past 2^24, where f32 are two apart)
                 }
                 bool hidden[COLS][4] = {};
                 if constexpr (MASKED) {

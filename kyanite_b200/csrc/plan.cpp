@@ -825,7 +825,9 @@ class Planner {
                  std::to_string(p.cache.heads) + " dim=" + std::to_string(p.cache.dim) + " capacity=" + std::to_string(p.cache.capacity) +
                  (info.prefix_at >= 0 ? " prefix=" + std::to_string(p.prefix.capacity) : "") + (p.half ? " f16" : " f32") + " cache " + dtype_name(cache.dtype) +
                  (p.many == 1 ? ", 128 rows at a time" : p.many == 2 ? ", the prefix 128 rows at a time" : "");
+        const double scratch = 4.0 * (plan.partial_floats + plan.part_floats + (plan.partial_floats ? plan.items : 0));
         push_step(std::move(s));
+        plan_.steps.back().alg_bytes -= scratch;
         return out;
     }
 

@@ -574,6 +574,48 @@ def test_one_hot_attention_copies_values():
     np.testing.assert_allclose(got[0, 0], (whole * scale)[last], rtol=2.0 ** -22)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("storage, dtype", [(I8, F16), (F16, F32)])
+def test_positions_far_into_a_large_cache(storage, dtype):
+    """Behind 4 GB of a cache: what is written there is what is read there, with a penalty on distance"""
+    sequences, heads, dim, capacity, tokens, window = 2, 2, 256, 2_200_000, 3, 40
+    cache = KvCache(0, sequences, heads, capacity, dim, storage)
+    assert cache.nbytes > 4 << 30
+    g = Graph()
+    c = g.cache(sequences, heads, capacity, dim, storage)
+    k, v = (g.input((sequences, 50, heads, dim)) for _ in range(2))
+    g.cache_write(c, k, v, g.input((sequences,), I32))
+    keys, values = (numbers(i, sequences, 50, heads, dim, dtype=F32) for i in (1, 2))
+    base = capacity - 50
+    with CudaExecutor(0, g, 1) as ex:
+        ex.set_cache(0, cache)
+        ex.evaluate([keys, values, np.array([base, base], np.int32)])
+    near = PlainCache(sequences, heads, 50, dim, storage)
+    near.write(keys, values, [0, 0])
+    for many in (tokens, 40):
+        q = numbers(9, sequences, many, 2 * heads, dim, dtype=dtype)
+        slopes = np.array([0.5, 0.25, 0.1, 0.01], np.float32)
+        got = attend(attention_graph(sequences, many, 2 * heads, heads, dim, capacity, dtype, storage, slopes=True, window=window), [cache],
+                     [q, np.array([base + 50 - many, base + 45 - many], np.int32), slopes]).astype(np.float64)
+        # (what lies in front is 0: keys whose scores are their distance alone, values of nothing)
+        held = np.concatenate([np.zeros_like(near.held), near.held], 3)
+        want, size, sums = plain_attention(q, held, [100 - many, 95 - many], slopes=slopes, window=window)
+        assert (np.abs(got - want).max(-1) <= attention_tolerance(dtype, size, sums, window)).all()
+
+
+@pytest.mark.gpu
+def test_no_sequences():
+    g = Graph()
+    c = g.cache(BATCH, 2, 30, 64)
+    x, start = g.input(shape(BATCH, 3, 2, 64), F16), g.input(shape(BATCH), I32)
+    y = g.cache_attention(x, g.cache_write(c, x, x, start), start)
+    g.output(y)
+    g.output(g.sample(g.view(g.value_cast(y, F32), shape(BATCH, 3 * 2 * 64)), g.input(shape(BATCH))))
+    with CudaExecutor(0, g, 0) as ex:
+        out = ex.evaluate([np.zeros((0, 3, 2, 64), np.float16), np.zeros(0, np.int32), np.zeros(0, np.float32)])
+    assert out[0].shape == (0, 3, 2, 64) and out[1].shape == (0,)
+
+
 # ------------------------------------------------------------------------------------------------ on the GPU: sampling
 
 
