@@ -1,8 +1,10 @@
 // A decoder's cache: writing the keys and values of new tokens into it, and reading all of it back as numbers.
 //
-//   scale = max_d |x_d| / 127,   q_d = round(x_d / scale)  (half to even),   read back as q_d * scale
+//   scale = max_d |x_d| * (1/127),   q_d = round(x_d / scale)  (half to even),   read back as q_d * scale
 //
-// per position and head, in f32 with IEEE divisions, so that any other program gets the same q and scale.  A row that holds an
+// per position and head, in f32 with each operation and the constant rounded to nearest, so that any other program gets the same q and scale.
+// (Not max / 127: what divides by a number that it knows beforehand multiplies, as tensor programs do, and one step of the scale moves the
+// numbers next to a half.)  A row that holds an
 // infinity or a NaN reads back as NaN throughout (its scale is NaN).
 //
 // Both are bound by memory: 8 channels a thread, so that a row's loads and stores are 16 bytes wide, and several rows a thread
@@ -80,7 +82,7 @@ __device__ __forceinline__ uint32_t four_of(const float* x, float scale, float r
 }
 // Rows for which that does not hold: the scale and eight numbers.  (A scale of few bits, of numbers next to nothing, may give more than 127)
 __device__ __noinline__ uint2 divided(const float* x, float most, float* scale) {
-    *scale = most < __int_as_float(0x7f800000) ? __fdiv_rn(most, 127.f) : __int_as_float(0x7fc00000);
+    *scale = most < __int_as_float(0x7f800000) ? __fmul_rn(most, 1.f / 127.f) : __int_as_float(0x7fc00000);
     float y[8];
 #pragma unroll 1
     for (int k = 0; k < 8; k++) y[k] = *scale > 0.f ? fminf(fmaxf(__fdiv_rn(x[k], *scale), -127.f), 127.f) : 0.f;
@@ -137,8 +139,7 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant_
 #pragma unroll
             for (int o = THREADS / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
             const float top = __uint_as_float(most);
-            float scale = top * (1.f / 127.f);
-            scale = fmaf(fmaf(-scale, 127.f, top), 1.f / 127.f, scale);   // (top / 127, by the same argument)
+            float scale = __fmul_rn(top, 1.f / 127.f);
             uint2 q;
             if (!(top > 1e-28f && top < 1e30f) || (__float_as_uint(scale) & 0x7fffffu) == 0x7fffffu) {
                 float y[8];

@@ -839,8 +839,8 @@ class Graph:
         """Extension: keys and values of up to `capacity` positions of each of `sequences` sequences, `heads` heads of `dim`
         channels, that outlive an evaluation.  Their storage is a `KvCache` of the same sizes that the program attaches to the
         executor (`CudaExecutor.set_cache`, by the order in which a graph's caches are made).  `dtype`: I8, whole numbers with
-        one f32 scale per position and head (scale = max|x| / 127, x read back as round(x / scale) * scale, rounding half
-        to even), or F16.  Only cache_write, cache_read and cache_attention take the value, of shape
+        one f32 scale per position and head (scale = max|x| * (1/127), all in f32, x read back as round(x / scale) * scale, rounding
+        half to even), or F16.  Only cache_write, cache_read and cache_attention take the value, of shape
         [2 (keys, values), sequences, heads, capacity, dim]."""
         if dtype not in (DType.I8, DType.F16):
             raise ValueError(f"a cache holds I8 or F16, got {dtype!r}")

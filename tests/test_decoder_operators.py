@@ -18,9 +18,9 @@ I8, F16, F32, I32 = DType.I8, DType.F16, DType.F32, DType.I32
 
 
 def quantise(x):
-    """(q, scale) of rows: scale = max|x| / 127 and q = round(x / scale), in f32 as IEEE has them"""
+    """(q, scale) of rows: scale = max|x| * (1/127) and q = round(x / scale), in f32 as IEEE has them"""
     x = x.astype(np.float32)
-    scale = (np.abs(x).max(-1, keepdims=True) / np.float32(127)).astype(np.float32)
+    scale = (np.abs(x).max(-1, keepdims=True) * (np.float32(1) / np.float32(127))).astype(np.float32)
     with np.errstate(divide="ignore", invalid="ignore"):
         q = np.where(scale > 0, np.clip(np.rint(x / scale), -127, 127), 0)
     return q, scale
