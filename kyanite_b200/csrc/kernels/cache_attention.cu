@@ -241,12 +241,13 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
     if (most > 0) {
         const int parts = (first_units + most - 1) / most;
         first_item = place / parts;
-        part = place % parts;
-        first_from = (int)((int64_t)first_units * part / parts);
-        todo = (int)((int64_t)first_units * (part + 1) / parts) - first_from;
+        part = place - first_item * parts;
+        const int least = first_units / parts, more = first_units - least * parts;   // the first `more` parts have one unit more
+        first_from = part * least + min(part, more);
+        todo = least + (part < more ? 1 : 0);
     } else {
         first_item = place / first_units;
-        first_from = place % first_units;
+        first_from = place - first_item * first_units;
         todo = each + ((int)blockIdx.x < longer ? 1 : 0);
     }
     int issued = 0, consumed = 0;
@@ -276,7 +277,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                 const Run r = run_of(next_span, ++next_run, next_from, until, warp, kWarps);
                 next_left = r.count;
                 const CacheParams& k = next_run ? p.cache : p.prefix;
-                next_tile = cache_tile(k, (next_run ? (int64_t)next_s * k.heads : 0) + next_item / row_tiles, r.first * kTile);
+                next_tile = cache_tile(k, (next_run ? (int64_t)next_s * k.heads : 0) + (row_tiles == 1 ? next_item : next_item / row_tiles), r.first * kTile);
             }
             if (tcp::elect_one()) {
                 tcp::mbar_expect_tx(bar_at + 8 * next_stage, G::kStage);
@@ -316,7 +317,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
     int u = u0;   // (equal ranges)
     for (int seq = first_seq, item = first_item, first_unit = first_from; todo > 0;) {
         // ---- an item, or the part of it that is this CTA's: units [first_unit, until) of its own
-        const int head = item / row_tiles, row0 = (item % row_tiles) * G::kRows;
+        const int head = row_tiles == 1 ? item : item / row_tiles, row0 = row_tiles == 1 ? 0 : (item % row_tiles) * G::kRows;
         const int units = units_of(span);
         const int until = min(units, first_unit + todo);
         if (!dead) issue();
