@@ -339,7 +339,13 @@ struct CacheRowsPlan {
 };
 CacheRowsPlan cache_attention_rows_plan(const CacheAttentionParams& p, int many);
 int launch_cache_attention_rows(const CacheAttentionParams& p, cudaStream_t stream);
-constexpr int kManyRows = 64, kManyKeys = 256;   // from which on rows are taken 128 at a time
+// From which on rows are taken 128 at a time (us by the step alone; 32 / 8 heads of 128 channels; rows x 128 against 16 at a time).
+// kManyRows, rows of a sequence that share keys: 16 rows, 16 x 2048 positions 51 / 30; 32 rows, 2 x 4096 29 / 26; 64 rows, 2 x 512
+// 21.7 / 19.4, 2 x 4096 33 / 33, 16 x 2048 54 / 111; 256 rows, 2 x 4096 45 / 92.
+// kManyKeys, positions of a prefix times the times that 16 rows at a time read them: a kernel and parts more are to be earned. At 2^19:
+// 16 sequences x 4096 45 / 36, 64 x 1024 70 / 49; at 2^20: 16 x 8192 55 / 59, 32 x 4096 44 / 60, 64 x 2048 69 / 67, 128 x 1024 97 / 83;
+// at 2^21: 64 x 4096 70 / 104, 128 x 2048 99 / 120.  (Of three executors side by side 2^20 is 1.2 to 2 times as fast, 2^19 1 to 1.4.)
+constexpr int kManyRows = 64, kManyKeys = 1 << 20;
 struct CacheAttentionPlan {
     int32_t grid;
     int64_t items, partial_floats;

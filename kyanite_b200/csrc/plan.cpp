@@ -797,7 +797,7 @@ class Planner {
         if (p.half && !p.cache.half && p.cache.dim <= 128) {
             const int64_t group = p.heads / p.cache.heads, rows = p.tokens * group;
             if (rows >= kManyRows) p.many = 1;
-            else if (p.prefix.dim && rows * p.cache.seqs >= kManyRows && p.prefix.capacity >= kManyKeys) p.many = 2;
+            else if (p.prefix.dim && rows * p.cache.seqs >= kManyRows && p.cache.seqs * (int64_t)p.cache.heads * ((rows + 15) / 16) * p.prefix.capacity >= kManyKeys) p.many = 2;
         }
         if (p.many != 0) {
             const CacheRowsPlan rows = cache_attention_rows_plan(p, p.many);

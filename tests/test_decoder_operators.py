@@ -436,8 +436,10 @@ def test_which_rows_are_taken_128_at_a_time():
     assert not plan_says("rows at a time", tokens=31, heads=4, kv_heads=2)
     for no in (dict(dtype=F32), dict(storage=F16), dict(dim=136)):
         assert not plan_says("rows at a time", tokens=100, heads=4, kv_heads=2, **no)
-    assert plan_says("the prefix 128 rows at a time", sequences=32, prefix=256)
-    assert not plan_says("rows at a time", sequences=31, prefix=256) and not plan_says("rows at a time", sequences=32, prefix=255)
+    # of a prefix: 64 rows of all sequences, and 2^20 positions read by 16 rows at a time
+    assert plan_says("the prefix 128 rows at a time", sequences=32, prefix=2 ** 14)
+    assert not plan_says("rows at a time", sequences=31, prefix=2 ** 15) and not plan_says("rows at a time", sequences=32, prefix=2 ** 14 - 1)
+    assert plan_says("the prefix 128 rows at a time", sequences=32, tokens=9, prefix=2 ** 13) and not plan_says("rows at a time", sequences=32, tokens=8, prefix=2 ** 13)
 
 
 @pytest.mark.gpu
@@ -491,10 +493,20 @@ def test_hidden_positions_of_many_rows_may_hold_anything(what):
     (40, 8, 2, 128, 1, 1000, None, {}), (70, 4, 4, 64, 1, 256, 100, {}), (9, 8, 1, 100, 2, 300, 0, {}), (33, 4, 1, 128, 1, 4000, 3999, dict(window=300)),
     (16, 16, 2, 64, 3, 700, 650, dict(slopes=True, softcap=15.0)), (70, 8, 1, 64, 1, 512, 512, {})])
 def test_prefix_of_all_sequences_at_once(sequences, heads, kv_heads, dim, tokens, prefix, length, more):
+    start = [(7 * s) % (60 - tokens) for s in range(sequences)]
+    start[1], start[2] = -1, -9                                     # sequences that see nothing (of their own, or at all)
+    check_attention(sequences, tokens, heads, kv_heads, dim, 60, start, prefix=prefix, prefix_length=length, count=[tokens] * (sequences - 1) + [0], **more)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sequences, heads, kv_heads, dim, tokens, prefix, length, more", [
+    (40, 8, 2, 128, 1, 13200, 1000, {}), (70, 4, 4, 64, 1, 3800, 100, {}), (70, 4, 4, 64, 1, 3800, None, {}), (9, 8, 1, 100, 2, 117000, 0, {}),
+    (33, 4, 1, 128, 1, 32000, 3999, dict(window=300)), (16, 16, 2, 64, 3, 17000, 650, dict(slopes=True, softcap=15.0)), (70, 8, 1, 64, 1, 15000, 512, {})])
+def test_long_prefix_of_all_sequences_at_once(sequences, heads, kv_heads, dim, tokens, prefix, length, more):
     sizes = dict(sequences=sequences, tokens=tokens, heads=heads, kv_heads=kv_heads, dim=dim, capacity=60, prefix=prefix)
     assert plan_says("the prefix 128 rows at a time", **sizes)
     start = [(7 * s) % (60 - tokens) for s in range(sequences)]
-    start[1], start[2] = -1, -9                                     # sequences that see nothing (of their own, or at all)
+    start[1], start[2] = -1, -9
     check_attention(sequences, tokens, heads, kv_heads, dim, 60, start, prefix=prefix, prefix_length=length, count=[tokens] * (sequences - 1) + [0], **more)
 
 
