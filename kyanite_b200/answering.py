@@ -34,10 +34,13 @@ class Answerer:
         self.held = np.zeros(self.batch, np.int32)      # positions of each sequence that the caches hold
         self.last_outputs = None
 
+    def _room(self, count):
+        if (self.held + np.asarray(count) > self.capacity).any():
+            raise ValueError(f"a sequence would have more than {self.capacity} positions")
+
     def _run(self, executor, ids, count, sampling):
         tokens = ids.shape[1]
-        if (self.held + count > self.capacity).any():
-            raise ValueError(f"a sequence would have more than {self.capacity} positions")
+        self._room(count)
         self.last_outputs = executor.evaluate([ids, self.held, count, configs.answer_rows(count, tokens), *sampling])
         self.held = self.held + count
         return self.last_outputs[0]
@@ -50,6 +53,7 @@ class Answerer:
         """Takes in a prompt for every sequence, behind what it holds already, and draws the token that follows each."""
         if len(prompts) != self.batch or min(len(x) for x in prompts) < 1:
             raise ValueError(f"expected {self.batch} prompts of one token and more")
+        self._room([len(x) for x in prompts])       # (all of it fits, or none goes in)
         sampling, found = self._sampling(uniform, temperature, top_k, top_p), np.zeros(self.batch, np.int32)
         for at in range(0, max(len(x) for x in prompts), self.piece):
             count = np.array([min(max(len(x) - at, 0), self.piece) for x in prompts], np.int32)
@@ -68,6 +72,10 @@ class Answerer:
 
     def answer(self, prompts: Sequence[Sequence[int]], tokens: int, uniform, **sampling) -> np.ndarray:
         """`tokens` tokens for every prompt, by random numbers `uniform` [tokens, batch] (or one for all)."""
+        if tokens < 1:
+            raise ValueError(f"expected one token and more, got {tokens}")
+        if len(prompts) == self.batch:
+            self._room([len(x) + tokens - 1 for x in prompts])
         uniform = np.broadcast_to(np.asarray(uniform, np.float32), (tokens, self.batch))
         out = [self.prompt(prompts, uniform[0], **sampling)]
         for u in uniform[1:]:

@@ -80,3 +80,18 @@ def test_answers_with_given_random_numbers():
             a.prompt([[1], [2], []], 0.5)
         with pytest.raises(ValueError):
             a.prompt([[1]], 0.5)
+
+
+@pytest.mark.gpu
+def test_what_does_not_fit_leaves_the_answerer_as_it_was():
+    """A prompt of several pieces, or an answer, that would pass the capacity is refused before its first piece goes in"""
+    with Answerer(0, batch=2, capacity=20, piece=8, math_mode=MATH_F32, **SMALL) as a:
+        with pytest.raises(ValueError, match="more than 20 positions"):
+            a.prompt([[1] * 21, [2]], 0.5)
+        assert a.held.tolist() == [0, 0]
+        with pytest.raises(ValueError, match="more than 20 positions"):
+            a.answer([[1] * 17, [2]], 5, 0.5)
+        with pytest.raises(ValueError, match="one token"):
+            a.answer([[1], [2]], 0, 0.5)
+        assert a.held.tolist() == [0, 0]
+        assert a.answer([[1] * 17, [2]], 4, 0.5).shape == (2, 4) and a.held.tolist() == [20, 4]
