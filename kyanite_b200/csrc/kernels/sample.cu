@@ -266,7 +266,7 @@ struct Slice {
     __device__ __forceinline__ u64 weight_bits(float x) const {
         const double d = (double)most - (double)fmaxf(x, least), magic = 6755399441055744.0;   // 1.5 x 2^52: a sum's low word is the number, rounded
         const double t = __fma_rn(d, rate, magic);
-        const int k = -__double2loint(t);   // (0 to 64 x 256)
+        const int k = -__double2loint(t);   // (0 to 400 x 256: up to 256 steps of the temperature from one f32 to the next, times log2(e))
         const double r = __fma_rn(d, rate, -(t - magic));   // 256 times the rest, up to 1/2 either way
         constexpr double kLn = 0.69314718055994531 / 256;
         double p = __fma_rn(r, kLn * kLn * kLn * kLn / 24, kLn * kLn * kLn / 6);
@@ -383,9 +383,14 @@ __global__ void __launch_bounds__(kCta, 2) sample_cluster_kernel(const __grid_co
         if (me == 0 && threadIdx.x == 0) p.out[r] = (int)first;
         return;
     }
-    row.rate = -256.0 * 1.4426950408889634074 / (double)temperature;
-    row.least = fmaxf(row.most - 44.f * temperature, -FLT_MAX);   // (e^-44 is 2^-63)
-    row.depth = fminf(2.f * (float)kBins / kDepth / temperature, 1e30f);
+    // No logit lies between the highest and the f32 below it.  Temperatures under 1/256 of that step leave weight to the highest alone, and count
+    // as that much: nothing in the exponent's arithmetic overflows then.  `least` is rounded down, so that what it stands for weighs e^-44
+    // and less, which is 2^-63, and never as much as the highest.
+    const float gap = row.most - nextafterf(row.most, -INFINITY);
+    const float heat = gap < INFINITY ? fmaxf(temperature, gap / 256.f) : temperature;
+    row.rate = -256.0 * 1.4426950408889634074 / (double)heat;
+    row.least = fmaxf(__fsub_rd(row.most, __fmul_ru(44.f, heat)), -FLT_MAX);
+    row.depth = fminf(2.f * (float)kBins / kDepth / heat, 1e30f);
     Cut cut{0, INT_MAX};
 
     // In the order of the index: what each piece weighs by `amount`, summed over the cluster; then the first index at which the

@@ -725,6 +725,53 @@ def test_sample_without_weights():
                 assert np.array_equal(got, plain_sample(logits, np.full(8, u, np.float32), **given)), (t, u)
 
 
+def sample_sideways(logits, uniform, **given):
+    """The same of logits whose rows do not lie together: the kernel that reads a row again and again"""
+    g = Graph()
+    names = ("temperature", "top_k", "top_p", "min_p")
+    x, u = g.input(logits.shape[::-1], DType.of(logits.dtype)), g.input(uniform.shape)
+    inputs = {n: g.input(given[n].shape, I32 if n == "top_k" else F32) for n in names if n in given}
+    g.output(g.sample(g.permute(x, [1, 0]), u, **inputs))
+    with CudaExecutor(0, g, 1) as ex:
+        return ex.evaluate([np.ascontiguousarray(logits.T), uniform] + [given[n] for n in inputs])[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("rule", [dict(), dict(top_k=50), dict(min_p=0.01), dict(top_p=1.0), dict(top_p=0.9), dict(top_k=3, min_p=1e-6)], ids=str)
+def test_sample_at_low_temperatures(dtype, rule):
+    """From where a logit's step is far above the temperature to where it is far below: logits of size 1 to 60000, some of them next to
+    the highest, forbidden tokens among them, an odd vocabulary"""
+    rng = np.random.default_rng(3)
+    vocab, sizes = 1001, (1, 20, 100, 1000, 60000)
+    logits = np.stack([np.float32(a) * (1 - rng.random(vocab, dtype=np.float32)) for a in sizes + tuple(-a for a in sizes)]).astype(dtype.np)
+    logits[:, rng.random(vocab) < 0.1] = -np.inf
+    logits[:, 500], logits[:, 77] = logits.max(-1), np.nan
+    for i in range(1, 30):                                               # down from the highest in steps
+        logits[:, 500 + 7 * i] = np.nextafter(logits[:, 500 + 7 * (i - 1)], np.array(-np.inf, dtype.np))
+    rows = len(logits)
+    given = {k: np.full(rows, v, np.int32 if k == "top_k" else np.float32) for k, v in rule.items()}
+    for t in (1e-45, 1e-30, 1e-8, 1e-7, 1e-6, 3e-6, 1e-5, 1e-4, 1e-3, 0.03):
+        given["temperature"] = np.full(rows, t, np.float32)
+        for u in (0.0, 0.25, 0.6, float(np.nextafter(np.float32(1), np.float32(0)))):
+            uniform = np.full(rows, u, np.float32)
+            want = plain_sample(logits, uniform, **given)
+            assert np.array_equal(sample(logits, uniform, **given), want), (t, u)
+            assert np.array_equal(sample_sideways(logits, uniform, **given), want), (t, u)
+
+
+@pytest.mark.gpu
+def test_tokens_that_weigh_nothing_are_not_drawn():
+    """As many tokens as a cluster holds, two steps below the highest, at a temperature that leaves e^-59 of its weight to each: together 2^-66 of it"""
+    logits = np.full((2, 8 * 46080), np.float32(20), np.float32)
+    step = np.float32(20) - np.nextafter(np.float32(20), np.float32(0))
+    logits[:, 1:] -= 2 * step
+    given = dict(temperature=np.full(2, step * np.float32(1.49 / 44), np.float32))
+    uniform = np.full(2, np.nextafter(np.float32(1), np.float32(0)), np.float32)
+    assert sample(logits, uniform, **given).tolist() == [0, 0]
+    assert sample(logits[:, :1 << 14], uniform, **given).tolist() == [0, 0]
+
+
 @pytest.mark.gpu
 def test_sample_reads_any_strides():
     """Logits of the last of several tokens, read in place, and a matrix that lies on its side"""
