@@ -494,7 +494,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             if constexpr (F32Q) s[n][i] = cap * tanhf(s[n][i]);
-                            else s[n][i] = cap - __fdividef(2.f * cap, 1.f + exp2_fast(fminf(s[n][i], 126.f)));
+                            else s[n][i] = cap - __fdividef(2.f * cap, 1.f + exp2_fast(tcp::min_keeping_nan(s[n][i], 126.f)));
                         }
                 }
                 if (p.slopes) {

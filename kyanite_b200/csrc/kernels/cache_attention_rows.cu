@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
                 x[2 * i + 1] = mul_pair(make_float2(__uint_as_float(v[i >> 3][c + 2]), __uint_as_float(v[i >> 3][c + 3])), make_float2(k.z, k.w));
             }
             if (p.softcap > 0.f) {
-                const auto capped = [&](float y) { return cap - __fdividef(2.f * cap, 1.f + exp2_approx(fminf(y, 126.f))); };   // tanh(y) = 1 - 2 / (1 + e^(2y))
+                const auto capped = [&](float y) { return cap - __fdividef(2.f * cap, 1.f + exp2_approx(min_keeping_nan(y, 126.f))); };   // tanh(y) = 1 - 2 / (1 + e^(2y))
 #pragma unroll
                 for (int i = 0; i < 32; i++) x[i] = make_float2(capped(x[i].x), capped(x[i].y));
             }

@@ -628,6 +628,60 @@ def test_no_sequences():
     assert out[0].shape == (0, 3, 2, 64) and out[1].shape == (0,)
 
 
+# ------------------------------------------------------------------------------------------------ on the GPU: attention, what nothing above asks for
+
+
+def held_after(cache, plain, writes):
+    """Writes rows (part, sequence, head, position, channel -> number) into both, position by position; their other numbers stay"""
+    _, sequences, heads, capacity, dim = plain.held.shape
+    g = Graph()
+    c = g.cache(sequences, heads, capacity, dim, plain.dtype)
+    k, v = (g.input((sequences, 1, heads, dim)) for _ in range(2))
+    g.cache_write(c, k, v, g.input((sequences,), I32), g.input((sequences,), I32))
+    with CudaExecutor(0, g, 1) as ex:
+        ex.set_cache(0, cache)
+        for (part, s, h, t, d), x in writes.items():
+            row = plain.held[:, :, :, t][:, :, None].copy()             # [2][sequences][1][heads][dim]
+            row[part, s, 0, h, d] = x
+            start, count = np.full(sequences, t, np.int32), (np.arange(sequences) == s).astype(np.int32)
+            ex.evaluate([row[0], row[1], start, count])
+            plain.write(row[0], row[1], start, count)
+
+
+def check_rows(got, q, plain, start, dtype, **more):
+    """Rows with infinities or NaN are those of the definition, number by number; the others within their tolerance, as if the
+    infinities, which are not in them, were 0"""
+    with np.errstate(invalid="ignore"):
+        want = plain_attention(q, plain.held, start, **more)[0]
+    finite = np.where(np.isfinite(plain.held), plain.held, 0)
+    _, size, sums = plain_attention(np.where(np.isfinite(q), q, 0), finite, start, **more)
+    allowed = attention_tolerance(dtype, size, sums, plain.capacity)[..., None]
+    got, there = got.astype(np.float64), np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), np.argwhere(np.isnan(got) != np.isnan(want))[:5]
+    assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    assert (np.abs(np.where(there, got, 0) - np.where(there, want, 0)) <= allowed).all()
+
+
+CAPPED = [dict(), dict(softcap=5.0), dict(softcap=30.0, window=50)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("more", CAPPED, ids=str)
+@pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("dtype, storage, tokens, heads, dim", [(F16, I8, 1, 4, 64), (F16, I8, 5, 4, 128), (F16, F16, 3, 4, 64), (F32, I8, 3, 4, 64), (F32, F16, 3, 2, 128), (F16, I8, 40, 4, 64),
+                                                                (F16, I8, 130, 2, 128)])
+def test_rows_of_an_8_bit_cache_and_queries_that_hold_no_numbers(dtype, storage, tokens, heads, dim, what, more):
+    """NaN stays NaN, with a cap and without: a query's, and a written row's (its scale is NaN) for whoever sees it"""
+    capacity, start = 240, [240 - tokens, 30]
+    cache, plain = filled(2, 2, capacity, dim, storage, 1)
+    q = numbers(9, 2, tokens, heads, dim, dtype=dtype)
+    q[1, tokens // 2, 1, 7] = what if storage == F16 and np.isnan(what) else np.nan
+    if storage == I8:
+        held_after(cache, plain, {(0, 0, 0, 200, 5): what, (0, 1, 1, 31, 0): what, (1, 1, 0, 20, 3): what})
+    got = attend(attention_graph(2, tokens, heads, 2, dim, capacity, dtype, storage, **more), [cache], [q, np.array(start, np.int32)])
+    check_rows(got, q, plain, start, dtype, **more)
+
+
 # ------------------------------------------------------------------------------------------------ on the GPU: sampling
 
 
