@@ -682,6 +682,21 @@ def test_rows_of_an_8_bit_cache_and_queries_that_hold_no_numbers(dtype, storage,
     check_rows(got, q, plain, start, dtype, **more)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, tokens, heads, dim", [(F16, 1, 2, 64), (F16, 1, 8, 128), (F16, 7, 8, 64), (F16, 3, 4, 192), (F16, 5, 8, 256), (F32, 1, 4, 64), (F32, 6, 4, 128), (F32, 2, 4, 256)])
+def test_infinite_values_of_a_16_bit_cache(dtype, tokens, heads, dim):
+    """Whoever sees an infinite value has it, whatever tile it is in; both of them, or a NaN, are a NaN"""
+    capacity, start = 300, [300 - tokens, 100]
+    cache, plain = filled(2, 2, capacity, dim, F16, 1)
+    held_after(cache, plain, {(1, 0, 0, 5, 0): np.inf, (1, 0, 0, 64, 1): -np.inf, (1, 0, 0, 299, 2): np.inf, (1, 0, 1, 130, 3): np.inf, (1, 0, 1, 131, 3): -np.inf,
+                              (1, 0, 1, 200, 9): np.nan, (1, 1, 0, 100, 4): 1e6, (1, 1, 0, 17, dim - 1): -1e6, (1, 1, 1, 250, 6): np.inf, (1, 1, 1, 101, 8): np.inf})
+    q = numbers(9, 2, tokens, heads, dim, dtype=dtype)
+    for more in (dict(), dict(window=150), dict(slopes=np.full(heads, 0.02, np.float32))):
+        g = attention_graph(2, tokens, heads, 2, dim, capacity, dtype, F16, **{k: v if k != "slopes" else True for k, v in more.items()})
+        got = attend(g, [cache], [q, np.array(start, np.int32)] + ([more["slopes"]] if "slopes" in more else []))
+        check_rows(got, q, plain, start, dtype, **more)
+
+
 # ------------------------------------------------------------------------------------------------ on the GPU: sampling
 
 
