@@ -465,8 +465,10 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
             const auto do_tile = [&](auto tag, int at, const uint8_t* stage) {
                 constexpr bool MASKED = decltype(tag)::value;
                 // ---- scores: 16 positions x 8 rows
-                // (8 rows: two sums, of every other group of channels, so that a product waits for the one before the last)
-                constexpr bool TWO = COLS == 1 && G::kGroups > 1;
+                // (8 rows: two sums, of every other group of channels, so that a product waits for the one before the last; of f32 queries and
+                // keys that may be infinite the queries' upper and lower halves)
+                constexpr bool TWO = COLS == 1 && G::kGroups > 1, BY_HALF = HALF && F32Q;
+                static_assert(TWO || !BY_HALF);
                 float s[COLS][4] = {}, other[4] = {};
 #pragma unroll
                 for (int k = 0; k < G::kGroups; k++) {
@@ -487,12 +489,13 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
 #pragma unroll
                         for (int n = 0; n < COLS; n++)
 #pragma unroll
-                            for (int half = 0; half < (F32Q ? 2 : 1); half++) mma(TWO && (k & 1) ? other : s[n], a, q[n][half][k][st][0], q[n][half][k][st][1]);
+                            for (int half = 0; half < (F32Q ? 2 : 1); half++) mma(TWO && (BY_HALF ? half : k & 1) ? other : s[n], a, q[n][half][k][st][0], q[n][half][k][st][1]);
                     }
                 }
                 if constexpr (TWO) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) s[0][i] += other[i];
+                    for (int i = 0; i < 4; i++)   // (an infinite key has its sign from the upper half)
+                        if (!BY_HALF || fabsf(s[0][i]) < INFINITY) s[0][i] += other[i];
                 }
                 float key_scale[2] = {1.f, 1.f}, value_scale[2] = {1.f, 1.f};
                 if constexpr (!HALF) {

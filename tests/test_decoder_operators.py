@@ -697,6 +697,20 @@ def test_infinite_values_of_a_16_bit_cache(dtype, tokens, heads, dim):
         check_rows(got, q, plain, start, dtype, **more)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("more", [dict(), dict(softcap=5.0)], ids=str)
+@pytest.mark.parametrize("dtype, tokens, heads, dim", [(F16, 1, 4, 64), (F16, 7, 8, 128), (F32, 1, 4, 64), (F32, 6, 4, 128), (F32, 2, 4, 256)])
+def test_infinite_keys_of_a_16_bit_cache(dtype, tokens, heads, dim, more):
+    """A score of minus infinity weighs nothing; one of infinity leaves no number; under a cap both are the cap"""
+    capacity, start = 300, [300 - tokens, 100]
+    for at, x in ((5, np.inf), (64, -np.inf), (299, np.inf), (130, -1e6)):
+        cache, plain = filled(2, 2, capacity, dim, F16, 1)
+        held_after(cache, plain, {(0, 0, 0, at, 2): x, (0, 1, 1, at // 3, 5): x})
+        q = numbers(9, 2, tokens, heads, dim, dtype=dtype)
+        got = attend(attention_graph(2, tokens, heads, 2, dim, capacity, dtype, F16, **more), [cache], [q, np.array(start, np.int32)])
+        check_rows(got, q, plain, start, dtype, **more)
+
+
 # ------------------------------------------------------------------------------------------------ on the GPU: sampling
 
 
