@@ -336,7 +336,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
                 for (int i = 0; i < 32; i++) x[i] = make_float2(capped(x[i].x), capped(x[i].y));
             }
             if (p.slopes) {
-                const float away = (float)(position + (run ? 0 : shared) - key0);
+                // (from the last position that the row sees, as in cache_attention.cu)
+                const float away = (float)(min(position, (int64_t)p.cache.capacity - 1) + (run ? 0 : shared) - key0);
 #pragma unroll
                 for (int i = 0; i < 32; i++) x[i].x -= slope * (away - (float)(2 * i)), x[i].y -= slope * (away - (float)(2 * i + 1));
             }

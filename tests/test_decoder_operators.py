@@ -711,6 +711,23 @@ def test_infinite_keys_of_a_16_bit_cache(dtype, tokens, heads, dim, more):
         check_rows(got, q, plain, start, dtype, **more)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("prefix", [0, 70])
+@pytest.mark.parametrize("dtype, tokens, heads", [(F16, 1, 4), (F16, 9, 4), (F32, 2, 4), (F16, 40, 4), (F16, 70, 2)])
+def test_penalties_far_behind_the_capacity(dtype, tokens, heads, prefix):
+    """Positions that f32, or a difference in 32 bits, do not hold: only how much further one key is than another decides"""
+    for start in ([2 ** 24 + 1, 2 ** 24 - 40], [2 ** 25 + 3, 2 ** 30 + 5], [2 ** 31 - 1, 2 ** 31 - tokens], [100, 99]):
+        check_attention(2, tokens, heads, 2, 64, 100, start, dtype, slopes=True, prefix=prefix)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sequences, prefix, length", [(70, 17000, 500), (32, 2 ** 15, 64)])
+def test_penalties_far_behind_the_capacity_with_a_long_prefix(sequences, prefix, length):
+    assert plan_says("the prefix 128 rows at a time", sequences=sequences, heads=8, kv_heads=2, dim=64, capacity=40, prefix=prefix)
+    start = [(2 ** 24 + 1, 2 ** 31 - 1, 39, 5, 2 ** 25 + 3)[i % 5] for i in range(sequences)]
+    check_attention(sequences, 1, 8, 2, 64, 40, start, slopes=True, prefix=prefix, prefix_length=length)
+
+
 # ------------------------------------------------------------------------------------------------ on the GPU: sampling
 
 
