@@ -27,18 +27,30 @@
 namespace kn {
 
 // One thread waits, through the same bounded wait every tensor-core kernel uses, on a barrier that nobody
-// arrives on: the wait runs out after `limit_cycles`, raises the status word and the kernel returns.  No tensor
-// memory, no copies in flight: nothing is left behind.  (kn_executor_selftest_wait_expiry)
-__global__ void wait_expiry_kernel(uint32_t* status, long long limit_cycles, uint32_t code) {
-    __shared__ __align__(8) unsigned long long bar;
+// arrives on: the wait runs out after `limit_cycles` and raises the status word.  Then a bulk copy of 256 bytes is under way, which has to be
+// waited for although the kernel has given up; the status is one higher if it has not come, or a plain wait does not know of
+// giving up.  No tensor memory: nothing is left behind.  (kn_executor_selftest_wait_expiry)
+__global__ void wait_expiry_kernel(uint32_t* status, long long limit_cycles, uint32_t code, const uint8_t* from) {
+    __shared__ __align__(8) unsigned long long bar[2];
+    __shared__ __align__(128) uint32_t to[64];
     __shared__ int abandon;
+    for (int i = threadIdx.x; i < 64; i += blockDim.x) to[i] = ~((const uint32_t*)from)[i];
     if (threadIdx.x == 0) {
-        tcp::mbar_init(tcp::smem_u32(&bar), 1);
+        for (auto& b : bar) tcp::mbar_init(tcp::smem_u32(&b), 1);
         abandon = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
-    if (threadIdx.x == 0) tcp::mbar_wait(tcp::smem_u32(&bar), 0, &abandon, status, code, limit_cycles);
+    if (threadIdx.x != 0) return;
+    const uint32_t never = tcp::smem_u32(&bar[0]), copied = tcp::smem_u32(&bar[1]);
+    bool right = !tcp::mbar_wait(never, 0, &abandon, status, code, limit_cycles);
+    tcp::mbar_expect_tx(copied, sizeof(to));
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tcp::smem_u32(to)), "l"(from),
+                 "r"((uint32_t)sizeof(to)), "r"(copied) : "memory");
+    right = tcp::mbar_drain(copied, 0, clock64()) && right && !tcp::mbar_wait(never, 0, &abandon, status, code) && !tcp::mbar_drain(never, 0, clock64(), limit_cycles);
+    for (int i = 0; i < 64; i++) right = right && to[i] == ((const uint32_t*)from)[i];
+    if (!right) atomicMax(status, code + 1);
 }
 
 namespace {
@@ -1240,7 +1252,7 @@ int kn_executor_selftest_wait_expiry(kn_executor* exec, uint32_t limit_us) {
         int khz = 0;
         KN_CUDA(cudaDeviceGetAttribute(&khz, cudaDevAttrClockRate, e.device));
         const long long cycles = (long long)limit_us * (long long)(khz > 0 ? khz : 2000000) / 1000ll;
-        kn::wait_expiry_kernel<<<1, 32, 0, e.stream>>>(e.status_dev, cycles, 99u);
+        kn::wait_expiry_kernel<<<1, 32, 0, e.stream>>>(e.status_dev, cycles, 99u, e.arena);
         KN_CUDA(cudaGetLastError());
         KN_CUDA(cudaMemcpyAsync(e.status_host, e.status_dev, 4, cudaMemcpyDeviceToHost, e.stream));
         KN_CUDA(cudaStreamSynchronize(e.stream));

@@ -885,7 +885,8 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
         }
     }
     // (given up: what is under way still writes to this CTA's shared memory)
-    for (; dead && consumed < issued; done_tile()) wait_tile();
+    if (dead)
+        for (const long long since = clock64(); consumed < issued; done_tile()) tcp::mbar_drain(bar_at + 8 * stage_at, phase, since);
 }
 
 // f(Geo, kernel) of the variant that takes p

@@ -99,8 +99,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* const gen = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t bars = base + G::kBars;
-    // per tile: queries are there; per stage full and empty, then per tile and parity of the block: scores complete, weights ready, values added
-    const uint32_t q_full = bars, full = bars + 16, empty = full + 8 * kStages, s_full = empty + 8 * kStages, p_ready = s_full + 32, pv_done = p_ready + 32;
+    // per tile: queries are there; per stage full and empty, then per tile and parity of the block: scores complete, weights ready, values added; last, all products
+    const uint32_t q_full = bars, full = bars + 16, empty = full + 8 * kStages, s_full = empty + 8 * kStages, p_ready = s_full + 32, pv_done = p_ready + 32, all_done = pv_done + 32;
     __shared__ uint32_t tmem_slot;
     __shared__ int abandon_flag, any_lo[2], any_hi[2], all_lo[2], all_hi[2];
     __shared__ float value_most[kStages][2];
@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
         mbar_init(q_full, 4), mbar_init(q_full + 8, 4);
         for (int i = 0; i < kStages; i++) mbar_init(full + 8 * i, 4), mbar_init(empty + 8 * i, 1);
         for (int i = 0; i < 4; i++) mbar_init(s_full + 8 * i, 1), mbar_init(p_ready + 8 * i, 4), mbar_init(pv_done + 8 * i, 1);
+        mbar_init(all_done, 1);
         abandon_flag = 0;
         for (int r = 0; r < 2; r++) any_lo[r] = all_hi[r] = 1 << 30, any_hi[r] = all_lo[r] = -(1 << 30);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -262,8 +263,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
                     }
                     mma_commit(pv_done + 16 * tile + 8 * b);
                 }
-                if (ok) mma_commit(empty + 8 * st);
+                if (ok && j + kStages < n) mma_commit(empty + 8 * st);   // (of the last ones nobody asks)
             }
+            // (whoever has given up, and when: nothing reads shared memory or writes tensor memory any more)
+            mma_commit(all_done);
+            mbar_drain(all_done, 0, clock64());
         }
         __syncwarp();
     } else {

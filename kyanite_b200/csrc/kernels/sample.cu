@@ -329,7 +329,8 @@ __global__ void __launch_bounds__(kCta, 2) sample_cluster_kernel(const __grid_co
     if (threadIdx.x == 0 && (n & 1)) x[n] = (T)-INFINITY;
     const float temperature = p.temperature ? p.temperature[r] : 1.f, uniform = p.uniform[r], top_p = p.top_p ? p.top_p[r] : 1.f, min_p = p.min_p ? p.min_p[r] : 0.f;
     const int top_k = p.top_k ? p.top_k[r] : 0;
-    if (whole > 0) tcp::mbar_wait(bar, 0, &sh.abandon, p.status, 72u);   // (given up: the row is wrong, the host learns of it)
+    // (given up: the host learns of it.  The copy is still waited for: what is counted below must not change meanwhile)
+    if (whole > 0 && !tcp::mbar_wait(bar, 0, &sh.abandon, p.status, 72u)) tcp::mbar_drain(bar, 0, clock64());
     __syncthreads();
     cluster.barrier_wait(std::move(started));
     // one number from each CTA; all get all of them

@@ -77,6 +77,14 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+// For a kernel that has given up: waits for a copy that is under way and would write to the memory of a CTA that has left, whatever the
+// flag that made the waits before it return says.  Bounded too, from `since` on: false if the copy has not come
+__device__ __forceinline__ bool mbar_drain(uint32_t bar, uint32_t parity, long long since, long long limit = kWaitCycles) {
+    while (!mbar_try_wait(bar, parity))
+        if (clock64() - since > limit) return false;
+    return true;
+}
+
 // The smaller of two; a NaN if either is one (fminf takes the other)
 __device__ __forceinline__ float min_keeping_nan(float a, float b) {
     float d;

@@ -893,6 +893,21 @@ def test_sample_reads_any_strides():
 
 
 @pytest.mark.gpu
+def test_copies_are_waited_for_by_a_kernel_that_has_given_up():
+    """The self-test's second part: behind a wait that ran out a copy is waited for, and has come; with the caches' executors usable afterwards"""
+    lib = _lib.load()
+    cache, plain = filled(2, 2, 40, 64, I8, 1)
+    q, start = numbers(9, 2, 1, 4, 64), np.array([39, 5], np.int32)
+    with CudaExecutor(0, attention_graph(), 1) as ex:
+        ex.set_cache(0, cache)
+        first = ex.evaluate([q, start])[0]
+        for _ in range(3):
+            assert lib.kn_executor_selftest_wait_expiry(ex._ptr, 200) == 7
+            assert b"(code 99)" in lib.kn_last_error()              # 100: a copy that did not come, or was not waited for
+            assert np.array_equal(ex.evaluate([q, start])[0], first)
+
+
+@pytest.mark.gpu
 def test_cache_handles_are_checked():
     g = attention_graph()
     inputs = [numbers(1, 2, 1, 4, 64), np.zeros(2, np.int32)]
