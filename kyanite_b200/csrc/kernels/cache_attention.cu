@@ -447,9 +447,6 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
             const int64_t zero = span.start + (run ? 0 : shared), end = run ? p.cache.capacity : shared;
             const auto high = [&](int t) { return cut(min(zero + t + 1, end)); };
             const auto low = [&](int t) { return p.window > 0 ? cut(zero + t - p.window + 1) : -(1 << 30); };
-            // The position that penalties are counted from: the last one that the row sees, which for rows behind the capacity is not its own (all
-            // scores of a row are higher by as much then, so that f32 holds them)
-            const auto last_of = [&](int t) { return (int)max(min(span.start + t, (int64_t)p.cache.capacity - 1), (int64_t)-(1 << 29)) + (run ? 0 : shared); };
             const int all_hi = high(t_first), any_hi = high(t_last), all_lo = low(t_last), any_lo = low(t_first);
             // whether some value of a tile is no finite number: 0 times all others is 0
             const auto holds_others = [&](const uint8_t* stage) {
@@ -522,10 +519,14 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                         }
                 }
                 if (p.slopes) {
+                    // (of sequences behind the capacity not from their positions: all scores of a row are higher by as much then, so that f32 holds
+                    // them.  Kept out of registers between tiles)
+                    int away = cut(min(span.start, (int64_t)p.cache.capacity - 1)) + (run ? 0 : shared) - at;
+                    asm volatile("" : "+r"(away));
 #pragma unroll
                     for (int n = 0; n < COLS; n++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) s[n][i] -= slope[n][i & 1] * (float)(last_of(t_of[n][i & 1]) - at - token[i >> 1]);   // (positions may be past 2^24, where f32 are two apart)
+                        for (int i = 0; i < 4; i++) s[n][i] -= slope[n][i & 1] * (float)(away + t_of[n][i & 1] - token[i >> 1]);   // (positions may be past 2^24, where f32 are two apart)
                 }
                 bool hidden[COLS][4] = {};
                 if constexpr (MASKED) {

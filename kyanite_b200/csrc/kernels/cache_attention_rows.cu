@@ -135,9 +135,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
     const int row = row0 + (threadIdx.x & (kRows - 1));
     Sight sight{};
     int64_t position = 0;   // behind the prefix
+    int counted = 0;        // what penalties count from, as in cache_attention.cu
     if (warp < 8 && row < rows) {
         const int s = seq_of(row), t = token_of(row);
         position = (int64_t)p.start[s] + t;
+        counted = max(min(p.start[s], p.cache.capacity - 1), -(1 << 30)) + t;
         sight.live = position >= 0 && (p.count == nullptr || t < p.count[s]);
         sight.high[0] = shared, sight.high[1] = cut(min(position + 1, (int64_t)p.cache.capacity));
         sight.low[0] = p.window > 0 ? max(cut(shared + position - p.window + 1), 0) : 0;
@@ -340,8 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
                 for (int i = 0; i < 32; i++) x[i] = make_float2(capped(x[i].x), capped(x[i].y));
             }
             if (p.slopes) {
-                // (from the last position that the row sees, as in cache_attention.cu)
-                const float away = (float)(min(position, (int64_t)p.cache.capacity - 1) + (run ? 0 : shared) - key0);
+                const float away = (float)(counted + (run ? 0 : shared) - key0);
 #pragma unroll
                 for (int i = 0; i < 32; i++) x[i].x -= slope * (away - (float)(2 * i)), x[i].y -= slope * (away - (float)(2 * i + 1));
             }
