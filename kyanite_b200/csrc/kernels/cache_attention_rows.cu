@@ -9,14 +9,16 @@
 //                   scales
 //   warp 12, a lane MMA issuer: the next block's scores go ahead of this block's products with the values, tile by tile
 //
-// Scores of a block are one of a tile's two accumulators of 64 columns in tensor memory; its weights, rounded to f16 and packed, take
-// their place and are the A operand of the second product, whose accumulator stays.  Scales of keys multiply scores, those of values
-// weights, in f32.  Weights go by a reference that no score is more than 2^8 above; it moves rarely, and then the thread rescales its
-// row (once the block before has been added).  Where the items are fewer than the SMs their keys are split over several
-// CTAs, and a second kernel joins the parts in order.
+// Scores of a block are one of a tile's two accumulators of 64 columns in tensor memory; its weights take their place as two halves of 11 bits
+// in f16, 32 columns each, and are the A operands of the second product, whose accumulator stays.  (22 bits, as cache_attention_kernel has
+// them: with the upper half alone results of f16 were 2.9e-4 from 64 bits, where their own rounding is 2.1e-4, and a sequence's
+// result depended on how many others there were.  The lower half costs 128.7 -> 146.0 us at the size below, 71.1 -> 73.5 behind a
+// prefix, step alone.)  Scales of keys multiply scores, those of values weights, in f32.  Weights go by a reference that no score is more
+// than 2^8 above; it moves rarely, and then the thread rescales its row (once the block before has been added).  Where the items are
+// fewer than the SMs their keys are split over several CTAs, and a second kernel joins the parts in order.
 //
-// Measured: 512 tokens of 2 sequences behind 4096 positions, 32 / 8 heads of 128 channels (73 GFLOP), 107 us: 682 TFLOP/s.  Bound by the
-// chain of a block's products and exponentials, each about 2 400 of its 3 000 cycles, that wait for one another.
+// Measured: 512 tokens of 2 sequences behind 4096 positions, 32 / 8 heads of 128 channels (73 GFLOP), step alone 146 us: 500 TFLOP/s.  Bound
+// by the chain of a block's products and exponentials that wait for one another.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -259,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
                     ok = mbar_wait(p_ready + 16 * tile + 8 * b, (uint32_t)((j >> 1) & 1), abandon, p.status, 85, kWaitCycles, kSleepNs);
                     if (!ok) break;
                     tc_fence_after();
-                    for (int s = 0; s < kKeys / 16; s++) {
-                        const uint64_t db = v_desc | (uint64_t)(((values + s * 16 * 128) & 0x3FFFFu) >> 4);
+                    for (int s = 0; s < 2 * (kKeys / 16); s++) {   // upper halves of the weights, then the lower ones
+                        const uint64_t db = v_desc | (uint64_t)(((values + s % (kKeys / 16) * 16 * 128) & 0x3FFFFu) >> 4);
                         mma_f16_weights(tmem + tile * 256 + 128, tmem + tile * 256 + b * kKeys + s * 8, db, idesc_o, (j | s) != 0 ? 1u : 0u);
                     }
                     mma_commit(pv_done + 16 * tile + 8 * b);
@@ -414,10 +416,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attention_rows_kernel(const
             }
 #pragma unroll
             for (int i = 0; i < 32; i++) {
-                const __half2 h = __floats2half2_rn(x[i].x, x[i].y);
-                v[0][i] = *(const uint32_t*)&h;
+                const __half2 hi = __floats2half2_rn(x[i].x, x[i].y);
+                const float2 back = __half22float2(hi), rest = add_pair(x[i], make_float2(-back.x, -back.y));
+                const __half2 lo = __floats2half2_rn(rest.x, rest.y);
+                v[0][i] = *(const uint32_t*)&hi, v[1][i] = *(const uint32_t*)&lo;
             }
             tmem_store_32(my_s, v[0]);
+            tmem_store_32(my_s + 32u, v[1]);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();

@@ -728,6 +728,61 @@ def test_penalties_far_behind_the_capacity_with_a_long_prefix(sequences, prefix,
     check_attention(sequences, 1, 8, 2, 64, 40, start, slopes=True, prefix=prefix, prefix_length=length)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("storage", [I8, F16])
+@pytest.mark.parametrize("sequences, tokens, heads, kv_heads, dim", [(40, 1, 8, 2, 64), (40, 1, 4, 4, 128), (9, 5, 8, 2, 256)])
+def test_weights_keep_more_bits_than_results(storage, sequences, tokens, heads, kv_heads, dim):
+    """Few keys whose values nearly cancel: of weights of 11 bits (2^-12 of each) the small results would be far off"""
+    check_weights(sequences, tokens, heads, kv_heads, dim, storage)
+
+
+def check_weights(sequences, tokens, heads, kv_heads, dim, storage):
+    capacity = tokens + 6
+    start = [s % 6 for s in range(sequences)]
+    cache, plain = filled(sequences, kv_heads, capacity, dim, storage, 1)
+    q = numbers(9, sequences, tokens, heads, dim)
+    got = attend(attention_graph(sequences, tokens, heads, kv_heads, dim, capacity, F16, storage, scale=0.3 / dim ** 0.5), [cache], [q, np.array(start, np.int32)]).astype(np.float64)
+    want, size, sums = plain_attention(q, plain.held, start, scale=0.3 / dim ** 0.5)
+    # the tolerance of results whose weights have 22 bits, and the result's own rounding, of which a number next to nothing has the least step
+    allowed = attention_tolerance(F32, size, sums, capacity)[..., None] + np.abs(want) * 2.0 ** -11 + 2.0 ** -25
+    assert (np.abs(got - want) <= allowed).all(), float((np.abs(got - want) / allowed).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sequences, tokens, heads, kv_heads, dim", [(3, 64, 2, 2, 64), (2, 40, 8, 2, 128), (2, 150, 2, 2, 100)])
+def test_weights_of_many_rows_keep_more_bits_than_results(sequences, tokens, heads, kv_heads, dim):
+    assert plan_says(", 128 rows at a time", sequences=sequences, tokens=tokens, heads=heads, kv_heads=kv_heads, dim=dim, capacity=tokens + 6)
+    check_weights(sequences, tokens, heads, kv_heads, dim, I8)
+
+
+@pytest.mark.gpu
+def test_results_do_not_depend_on_how_many_sequences_there_are():
+    """A prefix that 31 sequences read by 16 rows at a time, and 32 of them by 128: the same sequence has the same result but for a rounding"""
+    got, want = [], None
+    for n in (31, 32):
+        sizes = dict(heads=4, kv_heads=2, dim=64, capacity=40, prefix=2 ** 14)
+        assert plan_says("the prefix 128 rows at a time", sequences=n, **sizes) == (n == 32)
+        (cache, plain), (shared, held) = filled(n, 2, 40, 64, I8, 1), filled(1, 2, 2 ** 14, 64, I8, 30)
+        q = np.repeat(numbers(9, 1, 1, 4, 64), n, 0)
+        x = attend(attention_graph(sequences=n, **sizes), [cache, shared], [q, np.full(n, -1, np.int32), np.array([5], np.int32)])
+        assert (x == 0).all()                                       # (in front of position 0: sees nothing)
+        k = np.repeat(numbers(50, 1, 1, 2, 64), n, 0)
+        g = Graph()
+        c = g.cache(n, 2, 40, 64)
+        a, at = g.input((n, 1, 2, 64), F16), g.input((n,), I32)
+        g.cache_write(c, a, a, at)
+        with CudaExecutor(0, g, 1) as ex:
+            ex.set_cache(0, cache)
+            ex.evaluate([k, np.zeros(n, np.int32)])
+        plain.write(k, k, [0] * n)
+        x = attend(attention_graph(sequences=n, scale=0.04, **sizes), [cache, shared], [q, np.zeros(n, np.int32), np.array([5], np.int32)]).astype(np.float64)
+        assert (x == x[:1]).all()
+        got.append(x[0])
+        want, size, sums = plain_attention(q[:1], plain.held[:, :1], [0], scale=0.04, prefix=held.held, prefix_length=5)
+        allowed = attention_tolerance(F32, size, sums, 6)[..., None] + np.abs(want) * 2.0 ** -11 + 2.0 ** -25
+        assert (np.abs(x[:1] - want) <= allowed).all()
+
+
 # ------------------------------------------------------------------------------------------------ on the GPU: sampling
 
 
