@@ -339,12 +339,15 @@ struct CacheRowsPlan {
 };
 CacheRowsPlan cache_attention_rows_plan(const CacheAttentionParams& p, int many);
 int launch_cache_attention_rows(const CacheAttentionParams& p, cudaStream_t stream);
-// From which on rows are taken 128 at a time (us by the step alone; 32 / 8 heads of 128 channels; rows x 128 against 16 at a time).
-// kManyRows, rows of a sequence that share keys: 16 rows, 16 x 2048 positions 51 / 30; 32 rows, 2 x 4096 29 / 26; 64 rows, 2 x 512
-// 21.7 / 19.4, 2 x 4096 33 / 33, 16 x 2048 54 / 111; 256 rows, 2 x 4096 45 / 92.
-// kManyKeys, positions of a prefix times the times that 16 rows at a time read them: a kernel and parts more are to be earned. At 2^19:
-// 16 sequences x 4096 45 / 36, 64 x 1024 70 / 49; at 2^20: 16 x 8192 55 / 59, 32 x 4096 44 / 60, 64 x 2048 69 / 67, 128 x 1024 97 / 83;
-// at 2^21: 64 x 4096 70 / 104, 128 x 2048 99 / 120.  (Of three executors side by side 2^20 is 1.2 to 2 times as fast, 2^19 1 to 1.4.)
+// From which on rows are taken 128 at a time.  us of the step alone, and in brackets of three executors side by side; 32 / 8 heads of 128
+// channels, new tokens behind a cache; 128 against 16 rows at a time.
+// kManyRows, rows of a sequence that share keys: 32 rows, 2 x 4096 30.4 / 25.7 (21.5 / 18.9), 16 x 2048 58.9 / 64.6 (50 / 59); 64 rows, 2 x 512
+// 23.2 / 19.4 (8.9 / 14.3), 2 x 4096 34.8 / 33.2 (22.0 / 26.3), 16 x 2048 58 / 111 (50 / 103); 128 rows, 2 x 4096 36 / 46 (25 / 39).
+// kManyKeys, positions of a prefix times the times that 16 rows at a time read them: a kernel and parts more are to be earned.  Where a step is
+// alone that takes more of them the more sequences there are, side by side fewer: 2^20 lies between.  At 2^19: 16 sequences x 4096 47 / 37
+// (27 / 29), 32 x 2048 45 / 42 (26 / 36), 64 x 1024 72 / 49 (42 / 44), 128 x 512 99 / 65 (63 / 58); at 2^20: 16 x 8192 58 / 60 (33 / 50),
+// 32 x 4096 46 / 61 (27 / 54), 64 x 2048 73 / 68 (43 / 61), 128 x 1024 100 / 84 (63 / 75); at 2^21: 16 x 16384 79 / 97 (47 / 87), 32 x 8192
+// 56 / 99 (34 / 91), 64 x 4096 73 / 107 (45 / 98), 128 x 2048 101 / 122 (67 / 111).
 constexpr int kManyRows = 64, kManyKeys = 1 << 20;
 struct CacheAttentionPlan {
     int32_t grid;

@@ -10,7 +10,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cuda_runtime.h>
 
 #include "../kernels.h"
 
@@ -22,15 +21,9 @@ constexpr uint32_t kCacheZeros = 0x80808080u;   // four channels that are 0
 __host__ __device__ __forceinline__ int cache_swizzle(int row_bytes, int t) {
     return row_bytes % 128 == 0 ? (((t >> 2) & 3) << 1) ^ ((t & 1) << 2) : ((t >> 3) & 1) << 1;
 }
-// A row's first byte and its scale; part 0: keys, 1: values
+// The first byte of the tile that position t is in: keys, values, then, of an i8 cache, the keys' scales and the values'
 __host__ __device__ __forceinline__ uint8_t* cache_tile(const CacheParams& c, int64_t head /* of all sequences */, int t) {
     return c.base + (head * c.tiles + (t >> 4)) * c.tile_bytes;
-}
-__host__ __device__ __forceinline__ uint8_t* cache_row(const CacheParams& c, int part, int64_t head, int t) {
-    return cache_tile(c, head, t) + (part * kCacheTile + (t & 15)) * c.row_bytes;
-}
-__host__ __device__ __forceinline__ float* cache_scale(const CacheParams& c, int part, int64_t head, int t) {
-    return (float*)(cache_tile(c, head, t) + 2 * kCacheTile * c.row_bytes) + part * kCacheTile + (t & 15);
 }
 
 }  // namespace kn
