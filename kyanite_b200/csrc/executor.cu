@@ -143,6 +143,7 @@ struct Executor {
     std::vector<DenseChainParams> dense_runs;    // of plan->dense_runs
     std::vector<std::shared_ptr<CacheStorage>> caches;   // of plan->caches; null until attached
     std::vector<uint8_t> cache_used;             // ... by a step
+    bool ran = false, attached = false;          // the step list has run since its graphs were dropped; a cache has been attached since an evaluation
     Comm* comm = nullptr;              // not owned; AllReduce steps sum over its ranks (null: a world of one)
 
     ~Executor() {
@@ -203,6 +204,8 @@ struct Executor {
         // graphs captured with the previous storage would go on using it
         if (graph_exec) { cudaGraphExecDestroy(graph_exec); graph_exec = nullptr; }
         drop_eval_graphs();
+        ran = false;
+        attached = true;
         leave(caches[index]);
         caches[index] = std::move(c);
         patch_pointers(true);
@@ -477,7 +480,7 @@ struct Executor {
             for (auto& e : ev) cudaEventDestroy(e);
             return;
         }
-        if (use_graph()) {
+        if (use_graph() && (graph_exec || ran)) {
             if (!graph_exec) {
                 cudaGraph_t graph = nullptr;
                 KN_CUDA(cudaStreamBeginCapture(stream, cudaStreamCaptureModeThreadLocal));
@@ -496,10 +499,12 @@ struct Executor {
             KN_CUDA(cudaGraphLaunch(graph_exec, stream));
         } else {
             for (size_t i = 0; i < plan->steps.size(); i++) launch_at(i);
+            ran = true;
         }
     }
 
-    // The step list is captured into a CUDA graph and replayed, except when it contains collectives that go
+    // The step list is captured into a CUDA graph the second time that it runs (a first run, of a new executor or behind the attaching of a
+    // cache, is shorter launch by launch: one step of attention 27 us, with the capture 44; sampling 95 and 137) and replayed, except when it contains collectives that go
     // through NCCL: those are enqueued call by call, so that a rank that fails between steps cannot leave a
     // captured collective half-issued on the others.
     bool use_graph() const { return plan->opts.use_cuda_graph && !(plan->collectives > 0 && comm != nullptr && comm->world > 1); }
@@ -684,7 +689,8 @@ struct Executor {
         enter_caches();
         settle();
         staging_busy = true;
-        const bool graph = use_graph() && !profile;
+        const bool graph = use_graph() && !profile && !attached;   // (the first evaluation behind attaching: one by one, see use_graph)
+        attached = false;
         const bool later = graph && upload_in_graph();   // the graph's first node uploads
         for (size_t i = 0; i < pinned_in.size(); i++) {
             if (!bytes_in[i]) continue;

@@ -948,6 +948,31 @@ def test_sample_reads_any_strides():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("use_cuda_graph", [True, False])
+def test_caches_that_take_turns(use_cuda_graph):
+    """Three caches attached in turn, with one, two and three passes of either kind before the next: steps launched one by one, captured, and
+    replayed all read the cache that is attached, with inputs that change from pass to pass"""
+    held = [filled(2, 2, 40, 64, I8, seed) for seed in (1, 2, 3)]
+    with CudaExecutor(0, attention_graph(), 1, use_cuda_graph=use_cuda_graph) as ex:
+        for turn in range(9):
+            cache, plain = held[turn % 3]
+            ex.set_cache(0, cache)
+            for i in range(1 + turn // 3):
+                q, start = numbers(20 * turn + i, 2, 1, 4, 64), np.array([39 - turn, 5 + i], np.int32)
+                if turn % 2:
+                    got = ex.evaluate([q, start])[0]
+                else:
+                    ex.host_inputs[0][...], ex.host_inputs[1][...] = q, start
+                    ex.upload_inputs()
+                    ex.run_async()
+                    ex.download_outputs()
+                    ex.synchronize()
+                    got = ex.host_outputs[0].copy()
+                want, size, sums = plain_attention(q, plain.held, start)
+                assert (np.abs(got.astype(np.float64) - want).max(-1) <= attention_tolerance(F16, size, sums, 40)).all(), (turn, i)
+
+
+@pytest.mark.gpu
 def test_copies_are_waited_for_by_a_kernel_that_has_given_up():
     """The self-test's second part: behind a wait that ran out a copy is waited for, and has come; with the caches' executors usable afterwards"""
     lib = _lib.load()
