@@ -783,6 +783,63 @@ def test_results_do_not_depend_on_how_many_sequences_there_are():
         assert (np.abs(x[:1] - want) <= allowed).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, storage, sequences, tokens, heads, kv_heads, dim", [
+    (F16, I8, 3, 1, 4, 2, 64), (F16, I8, 2, 5, 8, 2, 128), (F16, F16, 2, 2, 4, 2, 80), (F32, I8, 3, 1, 4, 2, 64), (F32, F16, 2, 4, 6, 2, 100), (F16, I8, 2, 33, 4, 2, 64), (F16, I8, 2, 70, 2, 1, 100),
+    (F16, I8, 1, 129, 3, 3, 128)])
+def test_attention_takes_queries_of_any_strides(dtype, storage, sequences, tokens, heads, kv_heads, dim):
+    """Heads in front of tokens, the middle of wider rows (on and off 16 bytes), one row for all tokens, channels backwards, every other token"""
+    capacity = 2 * tokens + 30
+    cache, plain = filled(sequences, kv_heads, capacity, dim, storage, 1)
+    start = [tokens + 25 - i for i in range(sequences)]
+    for form in ("turned", "inside 8", "inside 1", "one", "backwards", "every other"):
+        dims = {"turned": (sequences, heads, tokens, dim), "inside 8": (sequences, tokens, heads, dim + 16), "inside 1": (sequences, tokens, heads, dim + 3),
+                "one": (sequences, 1, heads, dim), "every other": (sequences, 2 * tokens, heads, dim)}.get(form, (sequences, tokens, heads, dim))
+        x = numbers(9, *dims, dtype=dtype)
+        g = Graph()
+        c = g.cache(sequences, kv_heads, capacity, dim, storage)
+        a = g.input(dims, dtype)
+        view, q = {"turned": lambda: (g.permute(a, [0, 2, 1, 3]), x.transpose(0, 2, 1, 3)), "inside 8": lambda: (g.slice(a, 3, (8, dim + 8)), x[..., 8:dim + 8]),
+                   "inside 1": lambda: (g.slice(a, 3, (1, dim + 1)), x[..., 1:dim + 1]),
+                   "one": lambda: (g.broadcast(a, (sequences, tokens, heads, dim)), np.broadcast_to(x, (sequences, tokens, heads, dim))),
+                   "backwards": lambda: (g.flip(a, 3), x[..., ::-1]), "every other": lambda: (g.slice(a, 1, (0, 2 * tokens, 2)), x[:, ::2])}[form]()
+        g.output(g.cache_attention(view, c, g.input((sequences,), I32)))
+        assert "copy" not in plan_describe(g, 1)                        # read where it lies
+        got = attend(g, [cache], [x, np.array(start, np.int32)]).astype(np.float64)
+        want, size, sums = plain_attention(q, plain.held, start)
+        assert (np.abs(got - want).max(-1) <= attention_tolerance(dtype, size, sums, capacity)).all(), form
+
+
+@pytest.mark.gpu
+def test_many_rows_far_into_a_large_cache():
+    """Behind 4 GB of a cache, 128 rows at a time"""
+    heads, dim, capacity, tokens, window = 2, 128, 17_000_000, 64, 40
+    sizes = dict(sequences=1, tokens=tokens, heads=heads, kv_heads=heads, dim=dim, capacity=capacity)
+    assert plan_says(", 128 rows at a time", **sizes)
+    cache = KvCache(0, 1, heads, capacity, dim)
+    assert cache.nbytes > 2 * (4 << 30)
+    g = Graph()
+    c = g.cache(1, heads, capacity, dim)
+    k, v = (g.input((1, 120, heads, dim)) for _ in range(2))
+    g.cache_write(c, k, v, g.input((1,), I32))
+    keys, values, base = numbers(1, 1, 120, heads, dim, dtype=F32), numbers(2, 1, 120, heads, dim, dtype=F32), capacity - 120
+    with CudaExecutor(0, g, 1) as ex:
+        ex.set_cache(0, cache)
+        ex.evaluate([keys, values, np.array([base], np.int32)])
+    near = PlainCache(1, heads, 120, dim, I8)
+    near.write(keys, values, [0])
+    q, slopes = numbers(9, 1, tokens, heads, dim), np.array([0.3, 0.01], np.float32)
+    got = attend(attention_graph(slopes=True, window=window, **sizes), [cache], [q, np.array([base + 56], np.int32), slopes]).astype(np.float64)
+    want, size, sums = plain_attention(q, near.held, [56], slopes=slopes, window=window)
+    assert (np.abs(got - want).max(-1) <= attention_tolerance(F16, size, sums, window)).all()
+
+
+def test_short_prefixes_are_read_by_few_rows():
+    """The sizes of test_prefix_of_all_sequences_at_once: 16 rows at a time"""
+    for sequences, heads, kv_heads, dim, tokens, prefix in ((40, 8, 2, 128, 1, 1000), (70, 4, 4, 64, 1, 256), (9, 8, 1, 100, 2, 300), (33, 4, 1, 128, 1, 4000), (16, 16, 2, 64, 3, 700), (70, 8, 1, 64, 1, 512)):
+        assert not plan_says("rows at a time", sequences=sequences, tokens=tokens, heads=heads, kv_heads=kv_heads, dim=dim, capacity=60, prefix=prefix)
+
+
 # ------------------------------------------------------------------------------------------------ on the GPU: sampling
 
 
