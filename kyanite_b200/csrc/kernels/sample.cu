@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
             if (stays(x, i, w)) mass += w;
         }
         const u64 before = block_before(mass, sh.scratch), all = block_reduce(mass, sh.scratch, sum);
-        const double goal = (double)p.uniform[r] * (double)all;
+        const double goal = fmax((double)p.uniform[r] * (double)all, 0.0);
         u64 found = ~0ull, last = 0;
         u64 run = before;
         for (int i = from; i < until; i++) {
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
             const u64 w = weight(x);
             if (!stays(x, i, w)) continue;
             run += w;
-            if ((u64)i + 1 > last) last = (u64)i + 1;
+            if (w > 0 && (u64)i + 1 > last) last = (u64)i + 1;   // (of those that weigh something)
             if (found == ~0ull && (double)run > goal) found = (u64)i;
         }
         found = block_reduce(found, sh.scratch, least);
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kCta, 2) sample_cluster_kernel(const __grid_co
         if (me == 0 && threadIdx.x == 0) p.out[r] = -1;
         return;   // (all CTAs of the cluster; nobody reads another's memory any more)
     }
-    if (!(temperature > 0.f) || min_p > 1.f) {
+    if (!(temperature > 0.f) || !(min_p <= 1.f)) {
         // the first of the highest is all that stays
         uint32_t first = 0xffffffffu;
         for (int i = threadIdx.x; i < n; i += kCta)

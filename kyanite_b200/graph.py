@@ -957,7 +957,8 @@ class Graph:
         equals: the first top_k (I32; 0 or less: all) stay; of these the fewest that have top_p of their weight (1 or more: all);
         of these the ones that weigh at least min_p.  The first always stays.  Then, in the order of the index, the first token behind
         which more than uniform of the remaining weight lies.  Weights count in steps of 2^-44 of the highest.  Temperature 0
-        (or less): the highest logit, the lowest index among equals.  NaN counts as -infinity; a row with nothing else
+        (or less, or NaN), top_p NaN and min_p above 1 or NaN: the highest logit, the lowest index among equals.  uniform below 0 or NaN counts
+        as 0; of 1 and more it gives the last token that weighs anything.  NaN logits count as -infinity; a row with nothing else
         gives -1.  Of logits of +infinity each weighs 1 and all others 0."""
         s, d = self.shape_dtype(logits)
         if len(s) != 2 or d not in (DType.F32, DType.F16) or self[logits].kind in (OpKind.CACHE, OpKind.CACHE_WRITE):

@@ -973,6 +973,21 @@ def test_sample_at_low_temperatures(dtype, rule):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("draw", [sample, sample_sideways])
+def test_sample_by_numbers_out_of_range(draw):
+    """As the documentation has them, the same by both kernels; forbidden tokens in front, between and behind are not drawn"""
+    logits = np.full((7, 301), -np.inf, np.float32)
+    logits[:, [9, 40, 41, 200, 250]] = [1, 2, 2, np.nan, 0.5]
+    uniform = np.array([1, 2, np.inf, -0.5, -np.inf, np.nan, 0], np.float32)
+    assert draw(logits, uniform).tolist() == [250] * 3 + [9] * 4
+    assert draw(logits, uniform, top_k=np.full(7, 2, np.int32)).tolist() == [41] * 3 + [40] * 4
+    for name in ("temperature", "top_p", "min_p"):
+        assert draw(logits, uniform, **{name: np.full(7, np.nan, np.float32)}).tolist() == [40] * 7, name
+    assert draw(logits, uniform, min_p=np.full(7, 1.5, np.float32)).tolist() == [40] * 7
+    assert draw(logits, uniform, min_p=np.full(7, -1, np.float32)).tolist() == [250] * 3 + [9] * 4
+
+
+@pytest.mark.gpu
 def test_tokens_that_weigh_nothing_are_not_drawn():
     """As many tokens as a cluster holds, two steps below the highest, at a temperature that leaves e^-59 of its weight to each: together 2^-66 of it"""
     logits = np.full((2, 8 * 46080), np.float32(20), np.float32)
