@@ -190,7 +190,8 @@ KN_API int kn_executor_set_profile(kn_executor* exec, int enable);
 KN_API int kn_executor_last_profile(kn_executor* exec, char* buf, size_t cap, size_t* needed);
 /* Launches step `step` alone `launches` times back to back between one pair of CUDA events on the
  * executor's stream and returns the average duration of one launch in microseconds.  The step reads
- * and rewrites whatever its buffers currently hold.  (The per-step figures of `last_profile` include
+ * and rewrites whatever its buffers currently hold; a write into a cache goes to memory of the same size
+ * instead, so that the cache keeps what it holds.  (The per-step figures of `last_profile` include
  * the event and launch gaps of a one-by-one run; this one does not.)  No reference counterpart. */
 KN_API int kn_executor_time_step(kn_executor* exec, int step, int launches, float* microseconds);
 

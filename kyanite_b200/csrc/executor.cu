@@ -1119,13 +1119,36 @@ int kn_executor_time_step(kn_executor* exec, int step, int launches, float* micr
         KN_CHECK(launches >= 1 && launches <= 100000, KN_ERR_INVALID_ARG, "launch count out of range");
         kn::DeviceGuard guard(e.device);
         e.enter_caches();
+        kn::Step& s = e.plan->steps[step];
+        // What a write's operands hold now, which steps behind it may have used for something else, is not for the cache: it goes to memory
+        // of the same size
+        struct Away {
+            kn::CacheParams* cache = nullptr;
+            uint8_t* base = nullptr;
+            cudaStream_t stream = nullptr;
+            ~Away() {
+                if (cache == nullptr) return;
+                cudaStreamSynchronize(stream);
+                std::swap(cache->base, base);
+                cudaFree(base);
+            }
+        } away;
+        if (s.kind == kn::StepKind::CacheWrite) {
+            const size_t bytes = (size_t)kn::cache_bytes(s.cache_write.cache);
+            if (cudaError_t err = cudaMalloc((void**)&away.base, bytes)) {
+                cudaGetLastError();
+                kn::fail(KN_ERR_CUDA, "no device memory of a cache's " + std::to_string(bytes) + " bytes to time a write: " + cudaGetErrorString(err));
+            }
+            away.cache = &s.cache_write.cache, away.stream = e.stream;
+            std::swap(away.cache->base, away.base);
+        }
         cudaEvent_t a, b;
         KN_CUDA(cudaEventCreate(&a));
         KN_CUDA(cudaEventCreate(&b));
         try {
-            e.launch_step(e.plan->steps[step]);   // warm
+            e.launch_step(s);   // warm
             KN_CUDA(cudaEventRecord(a, e.stream));
-            for (int i = 0; i < launches; i++) e.launch_step(e.plan->steps[step]);
+            for (int i = 0; i < launches; i++) e.launch_step(s);
             KN_CUDA(cudaEventRecord(b, e.stream));
             KN_CUDA(cudaStreamSynchronize(e.stream));
             float ms = 0;

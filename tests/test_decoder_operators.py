@@ -1045,6 +1045,35 @@ def test_caches_that_take_turns(use_cuda_graph):
 
 
 @pytest.mark.gpu
+def test_timing_steps_leaves_caches_as_they_are():
+    """A write whose keys are computed, in memory that a later step uses again: timing it by itself does not write that into the cache"""
+    sequences, heads, dim, capacity = 2, 2, 64, 40
+    cache, plain = filled(sequences, heads, capacity, dim, I8, 1)
+    g = Graph()
+    c = g.cache(sequences, heads, capacity, dim)
+    x, start = g.input((sequences, 1, heads, dim), F32), g.input((sequences,), I32)
+    k = g.softmax(x, 3)
+    written = g.cache_write(c, k, k, start)
+    g.output(g.cache_read(written, F32))
+    g.output(g.softmax(g.softmax(g.softmax(x, 2), 1), 0))
+    a, at = numbers(5, sequences, 1, heads, dim, dtype=F32), np.array([7, 39], np.int32)
+    with CudaExecutor(0, g, 1) as ex:
+        ex.set_cache(0, cache)
+        first = ex.evaluate([a, at])[0].copy()
+        for again in range(2):
+            ex.evaluate([a, np.array([8, 50], np.int32)])           # (position 8 is the second evaluation's)
+            now = ex.evaluate([2 * a, np.array([9, 50], np.int32)])[0].copy()
+            for i in list(range(ex.step_count()[0]))[::-1] * 2:
+                assert ex.time_step(i, 3) > 0
+            reader = Graph()
+            reader.output(reader.cache_read(reader.cache(sequences, heads, capacity, dim), F32))
+            with CudaExecutor(0, reader, 1) as other:
+                other.set_cache(0, cache)
+                assert np.array_equal(other.evaluate([])[0], now)
+        assert np.array_equal(first[..., 10:, :], now[..., 10:, :]) and np.array_equal(first[..., :8, :], now[..., :8, :])
+
+
+@pytest.mark.gpu
 def test_copies_are_waited_for_by_a_kernel_that_has_given_up():
     """The self-test's second part: behind a wait that ran out a copy is waited for, and has come; with the caches' executors usable afterwards"""
     lib = _lib.load()
