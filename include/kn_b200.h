@@ -242,7 +242,7 @@ KN_API void kn_cache_destroy(kn_cache* cache);
 KN_API int kn_cache_bytes(const kn_cache* cache, uint64_t* bytes);
 KN_API int kn_executor_cache_count(const kn_executor* exec, int* n_caches);
 /* Attaches `cache` (NULL: none) as the graph's cache number `index`.  Waits for the executor's stream; not while an evaluation is in
- * flight.  One cache cannot stand for two of a graph's. */
+ * flight.  One cache cannot stand for two of a graph's.  What the executor has captured goes; its next pass launches step by step. */
 KN_API int kn_executor_set_cache(kn_executor* exec, int index, kn_cache* cache);
 
 /* Self-test of the bounded waits, with no counterpart in the reference.  Every barrier wait inside the

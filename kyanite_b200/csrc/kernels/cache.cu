@@ -93,8 +93,9 @@ __device__ __noinline__ uint2 divided(const float* x, float most, float* scale) 
 // THREADS threads a row (8 channels each), kEach rows a thread with their loads in flight together.  VEC: rows whose channels are
 // contiguous, 16-byte aligned and a multiple of 8.  A block takes positions of one head (and writes whole tiles), of few tokens heads of one
 // position (and reads what lies together).  7 prompts of up to 1500 tokens, 32 heads of 128 channels, f32 into i8 (270 MB): bound by
-// instructions while every row found its place by divisions and every number was divided (149 us); now 65 us.  Along the positions from
-// 16 tokens on: write and read of 7 x 1500 tokens take 146 us that way, 162 across the heads; of 16 x 16 156 and 155; of 32 x 1 305 and 300.
+// instructions while every row found its place by divisions and every number was divided (149 us); now 64 us.  Along the positions from
+// 16 tokens on (step alone, 32 heads of 128 channels, f16 into i8, along the positions / across the heads): 7 prompts of up to 1500 tokens 78.6 /
+// 94.8 us, 16 sequences x 64 9.6 / 10.6, 16 x 16 5.6 / 4.4, 32 x 4 7.7 / 4.2, 32 x 1 8.6 / 3.0.
 template <typename T, bool VEC, int THREADS>
 __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant__ CacheWriteParams p) {
     pdl_enter();

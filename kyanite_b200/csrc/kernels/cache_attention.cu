@@ -19,7 +19,8 @@
 //  * Numbers of 8 bits become f16 exactly (two instructions for two of them, cache.cuh), their scales multiply scores and weights
 //    in f32.  Weights, and f32 queries, are taken as two halves of 11 bits, a product each, and keep 22.
 //
-// Measured: 132 us for the sizes above (5.25 TB/s, 80 % of a copy), 53 us for one sequence of 131072 (276.8 MB, 80 %).
+// Measured, step alone: 133 us for the sizes above (5.2 TB/s, 80 % of a copy), 59 us for one sequence of 131072 (276.8 MB, 72 %; 54 of
+// three executors side by side, whose ends overlap).
 //
 // Softmax statistics and sums are f32.  A row's reference is not its maximum but one that no score is more than 2^8 above: it moves
 // rarely, and only then do lanes compare notes.
@@ -197,7 +198,9 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
     };
     const int grid = gridDim.x;
     int total = 0, most = 0;   // units; in a part, see below
-    const bool few = p.cache.seqs <= 64;   // every warp for itself then, two sequences a lane
+    // Up to 64 sequences every warp shares out for itself, two a lane, without a barrier.  (Step alone, all barriers and equal ranges -> this:
+    // 16 x 2048 26.6 -> 20.8 us, 64 x 300 28.4 -> 28.1, 64 x 8192 135.5 -> 133.3)
+    const bool few = p.cache.seqs <= 64;
     int mine[2] = {0, 0};
     if (few) {
 #pragma unroll
@@ -205,8 +208,8 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
             if (2 * lane + i < p.cache.seqs) mine[i] = units_at(2 * lane + i);
         total = __reduce_add_sync(0xffffffffu, mine[0] + mine[1]) * items;
         // Items in whole parts of up to `most` units, one part per CTA, where that is hardly longer than equal ranges: a CTA does not change
-        // items then.  (A change and a join are about as long as two units.  Step alone, equal ranges -> parts: 16 x 512 19.6 -> 14.3 us,
-        // 16 x 2048 25.8 -> 20.3, one of 131072 69.5 -> 58.7, 64 x 8192 133 -> 131.)
+        // items then.  (A change and a join are about as long as two units.  Step alone, equal ranges -> parts: 16 x 512 19.6 -> 14.5 us,
+        // 16 x 2048 25.8 -> 20.8, one of 131072 69.1 -> 58.7; 64 x 8192 133 and 133.)
         const int least = (total + grid - 1) / grid;
         for (int q = least; q <= least + 2 && most == 0; q++)
             if (__reduce_add_sync(0xffffffffu, (mine[0] + q - 1) / q + (mine[1] + q - 1) / q) * items <= grid) most = q;

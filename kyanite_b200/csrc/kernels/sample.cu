@@ -8,7 +8,9 @@
 // A row is read once, into the shared memory of a cluster of up to eight CTAs that share it.  Cuts are found from counts or weights of 1024
 // bins of the logits; a bin's tokens, if there are not too many, go to one CTA that ranks them all at once.  Weights are
 // computed in f64 by a table of 256 powers and four terms of a series: ten operations, where the general exp has some thirty.
-// Measured: 200 rows of 128256 f16 logits 57 us (51 MB: bound by f64 operations and issue, not memory), one of 32000 f32 4.8 us.
+// Measured, step alone (of three executors side by side): 200 rows of 128256 f16 logits of which all tokens stay 70 us (57), one of 32000 f32
+// 11.5 (4.8), with a top-k and a top-p 30 (11), greedy 3.8 (2.5).  51 MB of logits are 8 us of memory; issue slots are 56 % used, the f64 pipe
+// 24 %: most of the time warps wait at barriers (of a row's CTAs and the cluster), of which each cut has four to six more.
 // Rows that do not fit, or whose tokens do not lie together, are read again and again by one CTA.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
@@ -653,7 +655,7 @@ int cluster_of(const SampleParams& p, int* slice) {
     const auto tokens = [&](int ctas) { return ((p.vocab + ctas - 1) / ctas + unit - 1) / unit * unit; };
     int ctas = 1;
     // 64 KB a CTA, for two on an SM; and, of few rows, as many CTAs as have an SM's half, with 1024 tokens and more each.
-    // (Step alone: 200 x 128256 f16 70 us with 64 KB, 75 with 180; 16 x 128256 18.5 spread, 22.6 not; 8 x 32000 f32 12.9 and 15.7.)
+    // (Step alone: 200 x 128256 f16 70.6 us with 64 KB, 75.8 with 180; 16 x 128256 18.8 spread, 22.8 not; 8 x 32000 f32 12.9 and 15.8.)
     while (ctas < kMaxCluster && ((int64_t)tokens(ctas) * size > 64 * 1024 || (p.rows * ctas * 2 <= 2 * 148 && p.vocab / (2 * ctas) >= 1024))) ctas *= 2;
     *slice = tokens(ctas);
     return p.col_stride != 1 || (int64_t)*slice * size > 180 * 1024 || p.rows * ctas > INT_MAX ? 0 : ctas;

@@ -840,7 +840,7 @@ class Graph:
         channels, that outlive an evaluation.  Their storage is a `KvCache` of the same sizes that the program attaches to the
         executor (`CudaExecutor.set_cache`, by the order in which a graph's caches are made).  `dtype`: I8, whole numbers with
         one f32 scale per position and head (scale = max|x| * (1/127), all in f32, x read back as round(x / scale) * scale, rounding
-        half to even), or F16.  Only cache_write, cache_read and cache_attention take the value, of shape
+        half to even), or F16 (numbers past 65504 are infinities there).  Only cache_write, cache_read and cache_attention take the value, of shape
         [2 (keys, values), sequences, heads, capacity, dim]."""
         if dtype not in (DType.I8, DType.F16):
             raise ValueError(f"a cache holds I8 or F16, got {dtype!r}")
@@ -921,7 +921,8 @@ class Graph:
         sequence.  score = scale * q . k (default 1 / sqrt(dim)); then softcap * tanh(score / softcap) if `softcap` is not 0;
         then, with `slopes` (f32, one per query head), minus slope * distance.  With `window`, only positions less
         than that far away are seen.  Of a padded batch the first count[s] tokens count; the others, and tokens that see no
-        position (before 0, behind the capacity), get zeros."""
+        position (before 0, or a window behind the capacity), get zeros.  A score or a visible value that is NaN makes the row (or its channel) NaN,
+        with a cap or without; what a row does not see may hold anything."""
         qs, qd = self.shape_dtype(query)
         _, sequences, kv_heads, _, dim = self._cache_shape(cache)
         if len(qs) != 4 or qd not in (DType.F32, DType.F16) or (qs[0], qs[3]) != (sequences, dim) or self[query].kind in (OpKind.CACHE, OpKind.CACHE_WRITE):
