@@ -250,7 +250,8 @@ KN_API int kn_executor_set_cache(kn_executor* exec, int index, kn_cache* cache);
  * kernel return, and the next synchronising call reports KN_ERR_INTERNAL.  In normal operation no wait
  * expires, so this entry point makes one expire on purpose, harmlessly: a one-thread kernel waits
  * through the same routine, with a limit of `limit_us` microseconds (1 .. 100000), on a barrier in its own
- * shared memory that nothing arrives on.  It holds no tensor memory and has no copies in flight.
+ * shared memory that nothing arrives on.  It holds no tensor memory and has no copies in flight; behind
+ * the wait it begins one, which has to be waited for all the same (code 100 if it was not).
  * Returns KN_ERR_INTERNAL (the status path works, message "a kernel gave up waiting ... (code 99)") or
  * KN_OK (the expiry went unreported: a defect).  The status word is cleared and the executor stays usable. */
 KN_API int kn_executor_selftest_wait_expiry(kn_executor* exec, uint32_t limit_us);

@@ -322,6 +322,8 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
     }
     const float log2e = 1.4426950408889634f;
     const bool capped = p.softcap > 0.f;
+    // 2^x of how far a reference lies under another; of 16-bit caches no 0, so that a sum that is infinite stays so
+    const auto under = [](float x) { return HALF ? fmaxf(exp2_fast(x), 1.17549435e-38f) : exp2_fast(x); };
 
     bool dead = false;
     Span span = next_span;
@@ -579,7 +581,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
 #pragma unroll
                         for (int k = 0; k < 2; k++) {
                             const float top = fmaxf(ref[n][k], of_column(fmaxf(s[n][k], s[n][2 + k])));
-                            keep[k] = exp2_fast(ref[n][k] - top);
+                            keep[k] = under(ref[n][k] - top);
                             ref[n][k] = top;
                             above[n][k] = __fsub_rn(s[n][k], top);
                             above[n][2 + k] = __fsub_rn(s[n][2 + k], top);
@@ -753,7 +755,7 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const float m = most_of(8 * n + 2 * c + k);
-                times[n][k] = exp2_fast(ref[n][k] - m) * ((HALF ? 1.f : value_ref) / kWeight);
+                times[n][k] = under(ref[n][k] - m) * ((HALF ? 1.f : value_ref) / kWeight);
             }
         const bool whole = first_unit == 0 && until == units;
         const int64_t slot = 2 * (int64_t)blockIdx.x + (most > 0 || u == u0 ? 0 : 1);
@@ -863,12 +865,12 @@ cache_attention_kernel(const __grid_constant__ CacheAttentionParams p) {
                         float top = m;
 #pragma unroll
                         for (int i = 0; i < 8; i++) top = fmaxf(top, state[i].x);
-                        const float keep = exp2_fast(m - top);
+                        const float keep = under(m - top);
                         m = top;
                         all *= keep, v.x *= keep, v.y *= keep, v.z *= keep, v.w *= keep;
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
-                            const float f = i0 + i < parts ? exp2_fast(state[i].x - m) : 0.f;
+                            const float f = i0 + i < parts ? under(state[i].x - m) : 0.f;
                             if (i0 + i < parts) all += f * state[i].y, v.x += f * x[i].x, v.y += f * x[i].y, v.z += f * x[i].z, v.w += f * x[i].w;
                         }
                     }

@@ -4,7 +4,8 @@ Every per-sample tensor of a graph carries the batch size in its shape (`Size(fa
 exp > 0), samples never interact in the operations the executor runs, and the reference has no
 collective at all (it can only run one executor per device).  So a global batch is split on the host
 along each input's batch axis, every rank evaluates its shard with its own executor, and outputs are
-concatenated along their batch axis.  Inputs without a batch axis are replicated.
+concatenated along their batch axis.  Inputs without a batch axis are replicated.  A cache of a decoder (`Graph.cache`) of as many
+sequences as the batch has is a rank's own: each attaches storage for its shard.
 """
 from __future__ import annotations
 
